@@ -232,6 +232,67 @@ int lbw_qk_rmsnorm_rope_dt(const void* q_raw, const float* ss_q, const void* gam
                            const float* rope_sin, int rope_frames, int grid_h, int grid_w, int tok0, int rope_dtype,
                            void* stream);
 
+/* ---- packed sequences -------------------------------------------------------------------
+ * Batches of sequences of different lengths on one token axis (no padding), with grouped heads: the rotation by
+ * positions that are data, the per-head q/k norm with it, and the attention. Strides are in elements, the last
+ * dimension is contiguous, and pointers and strides are multiples of 16 bytes. None of these has a counterpart in
+ * the reference, whose path is one sequence on one (frame, h, w) grid per call. */
+enum lbw_dtype { LBW_BF16 = 0, LBW_FP16 = 1, LBW_FP32 = 2 };
+enum lbw_rope_layout {
+  LBW_ROPE_INTERLEAVED = 0, /* pair i = dims (2i, 2i + 1) */
+  LBW_ROPE_HALF = 1         /* pair i = dims (i, i + pairs) */
+};
+/* A rotation of `pairs` pairs (a multiple of 4, at most 128): pair i turns by position `axis[i]` times f_i, given as
+ * step[i] = round(f_i / (2 pi) * 2^64) mod 2^64, so that position * step wraps exactly at whole turns. */
+typedef struct {
+  int pairs, axes, layout, reserved;
+  unsigned char axis[128];
+  unsigned long long step[128];
+} lbw_rope_axes;
+/* out = x rotated, fp32 arithmetic, one rounding; dims beyond 2 * pairs are copied. x, out: [tokens, heads, head_dim]
+ * of lbw_dtype `dtype` (head_dim a multiple of 8, at most 256; out may be x). positions: [tokens, axes] int32 or int64
+ * (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does nothing. */
+int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, long long out_tok, long long out_head,
+                   long long tokens, int heads, int head_dim, int dtype, const void* positions, int pos_bits,
+                   long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream);
+/* One operand of lbw_qk_headnorm_rope: x [tokens, heads, head_dim] -> out [rows, heads, head_dim]; gamma [head_dim]
+ * of the tensors' type (or fp32 with gamma_f32), or NULL for no gain. */
+typedef struct {
+  const void* x;
+  void* out;
+  const void* gamma;
+  long long x_tok, x_head, out_row, out_head;
+  int heads, gamma_f32;
+} lbw_head_rows;
+/* Every head vector of q and k: x * rsqrt(mean(x^2) + eps) * gamma, then the rotation (rope NULL: none), fp32 with one
+ * rounding. With k_rows (int32 or int64 [tokens], k_rows_bits) token t's k goes to row k_rows[t] of k->out, and v, if
+ * given, is copied to row k_rows[t] of v->out (a cache of out_rows rows); a row outside [0, out_rows) is not written.
+ * Without k_rows the rows are the tokens. Two tokens with the same row: either is kept, head by head. */
+int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
+                         int head_dim, int dtype, float eps, const void* positions, int pos_bits, long long pos_tok,
+                         long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
+                         long long out_rows, void* stream);
+
+/* Attention of a batch of packed sequences: out_i = sum_j p_ij v_j with p = softmax over the visible keys of
+ * softmax_scale * q_i k_j, fp32 scores and sums. Sequence b has the query rows cu_q[b] .. cu_q[b + 1] - 1 and the keys
+ * cu_k[b] ..; there are cu_k[b + 1] - cu_k[b] of them, or k_lens[b] if k_lens is given (a cache with room for more: the
+ * rows past the length may hold anything). causal != 0: with nq queries and nk keys, query i sees keys
+ * 0 .. i + nk - nq. A row that sees no key gets zeros; rows of no sequence are left alone. cu_q, cu_k, k_lens: device
+ * int32, read when the kernels run (a captured graph may be replayed with others); starts and lengths that do not fit
+ * the tensors are cut to what does.
+ * q, out: [tq, hq, head_dim]; k, v: [tk, hk, head_dim]; hq a multiple of hk, query head h uses kv head h / (hq / hk);
+ * head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A non-finite value in a visible key or value reaches the
+ * rows that see it; in a value row it also reaches rows of the same sequence that stand before it by less than 128 keys.
+ * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
+ * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap. */
+int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
+                                   long long* bytes);
+int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const void* k, long long k_tok,
+                         long long k_head, const void* v, long long v_tok, long long v_head, void* out,
+                         long long out_tok, long long out_head, const int* cu_q, const int* cu_k, const int* k_lens,
+                         int n_seqs, long long tq, long long tk, int hq, int hk, int head_dim, int dtype, int causal,
+                         float softmax_scale, int max_q, void* workspace, long long ws_bytes, void* stream);
+
 /* ---- MXFP8 -------------------------------------------------------------------------------- */
 /* Quantise bf16 x [rows, k] (k % 128 == 0) to E4M3 data [rows, k] and E8M0 scales in the tiled
  * layout (rows padded to 128, 512-byte atoms of 128 rows x 4 scales); optionally also the

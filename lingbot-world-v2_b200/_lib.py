@@ -66,6 +66,11 @@ SIGNATURES = {
     "lbw_mx_linear_rowss": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp], _i),
     "lbw_mx_linear_residual_film": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp], _i),
     "lbw_mx_linear_act": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp], _i),
+    "lbw_axial_rope": ([_vp, _ll, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _vp, _i, _ll, _ll, _vp, _i, _vp], _i),
+    "lbw_qk_headnorm_rope": ([_vp, _vp, _vp, _ll, _i, _i, _f, _vp, _i, _ll, _ll, _vp, _vp, _i, _ll, _vp], _i),
+    "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, ctypes.POINTER(_ll)], _i),
+    "lbw_packed_attention": ([_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _ll, _ll,
+                              _i, _i, _i, _i, _i, _f, _i, _vp, _ll, _vp], _i),
     "lbw_vae_conv": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "lbw_vae_conv_rms": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
     "lbw_vae_rms_silu": ([_vp, _ll, _i, _i, _vp, _i, _vp, _vp], _i),
@@ -130,13 +135,20 @@ CALLS = [0]
 def check(rc, what, launches=1):
     """Raises on a non-zero status; on success counts `launches` kernels enqueued by the call."""
     if rc == LBW_OK:
-        if what not in ("device status", "lbw_init", "lbw_destroy", "attention_tail_plan"):
+        if what not in ("device status", "lbw_init", "lbw_destroy", "attention_tail_plan",
+                        "packed_attention_workspace"):
             CALLS[0] += launches
         return
     msg = f"{what}: {last_error()} (status {rc})"
     if rc in (LBW_ERR_INVALID, LBW_ERR_SHAPE, LBW_ERR_ALIGN, LBW_ERR_UNSUPPORTED):
         raise ValueError(msg)
     raise LbwError(msg)
+
+
+class HeadRows(ctypes.Structure):
+    """lbw_head_rows (include/lbw.h)."""
+    _fields_ = [("x", _vp), ("out", _vp), ("gamma", _vp), ("x_tok", _ll), ("x_head", _ll), ("out_row", _ll),
+                ("out_head", _ll), ("heads", _i), ("gamma_f32", _i)]
 
 
 def ptr(t):

@@ -11,10 +11,15 @@ served by the sm_100a chunk-attention kernel (liblbw.so: lbw_chunk_attention).
   cross_attention_dedup(q, k, v, bias, kc)        attention.py:532-554 (token-major K/V here)
 
 q/k/v are [1, L, n, d] (or [L, n, d]) bf16 CUDA tensors with d = 128; outputs are [1, Lq, n, d] bf16.
+
+  packed_attention(q, k, v, cu_q, cu_k, ...)      no counterpart there: a batch of sequences of different lengths on
+                                                  one token axis, causal or not, grouped heads, cached keys, bf16 or
+                                                  fp16, d = 64 or 128 (lbw_packed_attention; see kernels)
 """
 import torch
 
 from . import kernels
+from .kernels import packed_attention, packed_attention_workspace  # noqa: F401
 
 
 def _lq(q):

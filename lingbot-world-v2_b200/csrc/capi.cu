@@ -82,6 +82,27 @@ int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, 
   return LBW_OK;
 }
 
+int make_tmap_3d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, uint64_t n0, uint64_t n1, uint64_t n2,
+                 uint64_t stride1, uint64_t stride2, uint32_t box1, uint32_t box2) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(LBW_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (!aligned(base, 16)) return set_error(LBW_ERR_ALIGN, "TMA base address not 16-byte aligned");
+  if (n0 == 0 || n1 == 0 || n2 == 0) return set_error(LBW_ERR_SHAPE, "empty TMA tensor");
+  if (n1 == 1) stride1 = n0;  // the stride of an axis of one element is never used
+  if (n2 == 1) stride2 = n0;
+  if (stride1 < n0 || stride2 < n0) return set_error(LBW_ERR_SHAPE, "strides smaller than a row of %d", (int)n0);
+  if ((stride1 * 2) % 16 != 0 || (stride2 * 2) % 16 != 0)
+    return set_error(LBW_ERR_ALIGN, "TMA strides not multiples of 16 bytes");
+  cuuint64_t dims[3] = {n0, n1, n2};
+  cuuint64_t strides[2] = {stride1 * 2, stride2 * 2};
+  cuuint32_t box[3] = {64, box1, box2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, dtype, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(LBW_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return LBW_OK;
+}
+
 int num_sms() {
   static int cache[64] = {0};
   int dev = 0;

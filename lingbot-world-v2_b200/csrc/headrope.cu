@@ -1,0 +1,380 @@
+// Row kernels over (token, head) vectors: the rotation by positions on several axes (lbw_axial_rope), and the RMSNorm
+// of every q and k head with that rotation in the same pass (lbw_qk_headnorm_rope).
+//
+// For one head vector x of D values, R rotated pairs and the token's integer positions pos[axis]:
+//   n_d  = x_d * rsqrt(mean_d(x_d^2) + eps) * gamma_d            (norm form; n = x otherwise)
+//   t_i  = pos[axis(i)] * f_i                                    (angle of pair i)
+//   y    = (a cos t - b sin t, a sin t + b cos t)                for the pair (a, b) of n; dims beyond 2R: y = n
+// All in fp32 with one rounding to the output type. The angle is reduced exactly: with F_i = round(f_i / 2pi * 2^64)
+// the integer product pos * F_i mod 2^64 IS the angle in 2^-64 turns, for any 64-bit position of either sign, so far
+// positions lose nothing (an fp32 product pos * f_i is 6e-3 rad off at position 100,000).
+//
+// Bound: bytes (each value read once and written once, ~7 flops each). A head is D / 8 "units" of 8 values, one per
+// lane: unit u holds the pairs 4u .. 4u + 3, which are 8 neighbouring values (interleaved pairs: one 16-byte access)
+// or two runs of 4 values R apart (half layout: two 8-byte accesses), so a pair never crosses lanes and the only
+// exchange is the norm's sum over the head's 8, 16 or 32 lanes. A lane has the same unit of every head that it visits:
+// it computes its four angles once for a token and uses them for all of its heads.
+#include <cuda_fp16.h>
+
+#include "host_common.cuh"
+#include "lbw_common.cuh"
+
+namespace lbw {
+
+namespace hr {
+constexpr int THREADS = 128;
+constexpr int UN = 4;  // heads loaded ahead by a lane group
+}  // namespace hr
+
+// One group of heads of every token: q, k or v. Strides in elements.
+struct HeadSeg {
+  const void* x;
+  void* out;
+  const void* gamma;  // null: no gain
+  long long xs_tok, xs_head, os_tok, os_head;
+  int heads;
+  int gamma_f32;
+  int mode;     // 0: norm (if the kernel norms) + rotation, 1: plain copy
+  int scatter;  // 1: the token's output row is rows[token]
+};
+
+struct HeadArgs {
+  HeadSeg seg[3];
+  long long tokens;
+  int dim, units, group;  // units = dim / 8, group = lanes of a head (8, 16 or 32)
+  int chunk, chunks;      // heads per work item, items per token
+  float eps;
+  const void* pos;
+  int pos_bits;
+  long long ps_tok, ps_axis;
+  const void* rows;
+  int rows_bits;
+  long long out_rows;
+  lbw_rope_axes rope;
+};
+
+template <typename T>
+struct Vec8;  // 8 values of T as raw registers
+template <>
+struct Vec8<float> {
+  float4 a, b;
+};
+template <>
+struct Vec8<__nv_bfloat16> {
+  uint2 a, b;
+};
+template <>
+struct Vec8<__half> {
+  uint2 a, b;
+};
+
+template <typename T, bool HALF>
+LBW_DEV void load8(Vec8<T>& r, const T* p, int o0, int o1) {
+  if constexpr (sizeof(T) == 2 && !HALF) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p + o0);
+    r.a = make_uint2(v.x, v.y);
+    r.b = make_uint2(v.z, v.w);
+  } else {
+    r.a = *reinterpret_cast<const decltype(r.a)*>(p + o0);
+    r.b = *reinterpret_cast<const decltype(r.b)*>(p + o1);
+  }
+}
+template <typename T, bool HALF>
+LBW_DEV void store8(const Vec8<T>& r, T* p, int o0, int o1) {
+  if constexpr (sizeof(T) == 2 && !HALF) {
+    *reinterpret_cast<uint4*>(p + o0) = make_uint4(r.a.x, r.a.y, r.b.x, r.b.y);
+  } else {
+    *reinterpret_cast<decltype(r.a)*>(p + o0) = r.a;
+    *reinterpret_cast<decltype(r.b)*>(p + o1) = r.b;
+  }
+}
+
+LBW_DEV void unpack8(const Vec8<float>& r, float (&f)[8]) {
+  f[0] = r.a.x, f[1] = r.a.y, f[2] = r.a.z, f[3] = r.a.w;
+  f[4] = r.b.x, f[5] = r.b.y, f[6] = r.b.z, f[7] = r.b.w;
+}
+LBW_DEV void pack8(Vec8<float>& r, const float (&f)[8]) {
+  r.a = make_float4(f[0], f[1], f[2], f[3]);
+  r.b = make_float4(f[4], f[5], f[6], f[7]);
+}
+LBW_DEV void unpack8(const Vec8<__nv_bfloat16>& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+LBW_DEV void pack8(Vec8<__nv_bfloat16>& r, const float (&f)[8]) {
+  r.a = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+  r.b = make_uint2(pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+LBW_DEV void unpack8(const Vec8<__half>& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+LBW_DEV uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+LBW_DEV void pack8(Vec8<__half>& r, const float (&f)[8]) {
+  r.a = make_uint2(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]));
+  r.b = make_uint2(pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
+}
+
+LBW_DEV float load_as_float(const float* p) { return *p; }
+LBW_DEV float load_as_float(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+LBW_DEV float load_as_float(const __half* p) { return __half2float(*p); }
+
+LBW_DEV long long load_index(const void* p, int bits, long long i) {
+  return bits == 64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
+}
+
+// Heads [h0, h1) of one segment of one token, `slots` heads at a time per warp and UN of those loaded ahead (the loads
+// of all UN come before the first store: input and output may be the same tensor).
+template <typename T, bool NORM, bool HALF>
+LBW_DEV void head_run(const HeadArgs& a, const HeadSeg& g, long long tok, long long row, int h0, int h1, int sub, int u,
+                      int slots, int o0, int o1, bool rotated, const float (&c)[4], const float (&s)[4],
+                      const float (&gain)[8]) {
+  const T* xt = reinterpret_cast<const T*>(g.x) + tok * g.xs_tok;
+  T* ot = reinterpret_cast<T*>(g.out) + row * g.os_tok;
+  const bool on = u < a.units;
+  const float inv_d = 1.f / (float)a.dim;
+  for (int h = h0 + sub; h - sub < h1; h += slots * hr::UN) {
+    Vec8<T> r[hr::UN];
+#pragma unroll
+    for (int i = 0; i < hr::UN; ++i) {
+      r[i] = Vec8<T>{};
+      if (on && h + i * slots < h1) load8<T, HALF>(r[i], xt + (h + i * slots) * g.xs_head, o0, o1);
+    }
+#pragma unroll
+    for (int i = 0; i < hr::UN; ++i) {
+      if (h - sub + i * slots >= h1) break;  // warp-uniform
+      if (g.mode == 0 && (NORM || rotated)) {  // (what is only copied keeps its bits, a NaN's too)
+        float f[8];
+        unpack8(r[i], f);
+        if constexpr (NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+          for (int o = a.group >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float k = rsqrtf(fmaf(ss, inv_d, a.eps));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = f[e] * k * gain[e];
+        }
+        if (rotated) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const int lo = HALF ? p : 2 * p, hi = HALF ? p + 4 : 2 * p + 1;
+            const float x0 = f[lo], x1 = f[hi];
+            f[lo] = x0 * c[p] - x1 * s[p];
+            f[hi] = x0 * s[p] + x1 * c[p];
+          }
+        }
+        pack8(r[i], f);
+      }
+      if (on && h + i * slots < h1) store8<T, HALF>(r[i], ot + (h + i * slots) * g.os_head, o0, o1);
+    }
+  }
+}
+
+// Work item = (token, chunk of the token's q | k | v heads), one warp each, grid-stride.
+template <typename T, bool NORM, bool HALF>
+__global__ void __launch_bounds__(hr::THREADS) head_rope_kernel(const __grid_constant__ HeadArgs a) {
+  __shared__ unsigned long long step[128];
+  __shared__ unsigned char axis[128];
+  for (int i = threadIdx.x; i < a.rope.pairs; i += hr::THREADS) {
+    step[i] = a.rope.step[i];
+    axis[i] = a.rope.axis[i];
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int slots = 32 / a.group;
+  const int u = lane & (a.group - 1), sub = lane / a.group;
+  const bool rotated = 4 * u < a.rope.pairs;
+  const int o0 = HALF && rotated ? 4 * u : 8 * u;
+  const int o1 = HALF && rotated ? a.rope.pairs + 4 * u : 8 * u + 4;
+  float gain[2][8];
+  if constexpr (NORM) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = e < 4 ? o0 + e : o1 + e - 4;
+        gain[w][e] = 1.f;
+        if (a.seg[w].gamma && u < a.units)
+          gain[w][e] = a.seg[w].gamma_f32 ? reinterpret_cast<const float*>(a.seg[w].gamma)[d]
+                                          : load_as_float(reinterpret_cast<const T*>(a.seg[w].gamma) + d);
+      }
+  }
+  const int hq = a.seg[0].heads, hk = a.seg[1].heads, hv = a.seg[2].heads;
+  const long long items = a.tokens * a.chunks;
+  const long long stride = (long long)gridDim.x * (hr::THREADS / 32);
+  for (long long it = (long long)blockIdx.x * (hr::THREADS / 32) + (threadIdx.x >> 5); it < items; it += stride) {
+    const long long tok = it / a.chunks;
+    const int lo = (int)(it - tok * a.chunks) * a.chunk;
+    const int hi = min(lo + a.chunk, hq + hk + hv);
+    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (rotated && lo < hq + hk) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int i = 4 * u + p;
+        const long long ps = load_index(a.pos, a.pos_bits, tok * a.ps_tok + axis[i] * a.ps_axis);
+        const unsigned long long turns = (unsigned long long)ps * step[i];
+        sincospif((float)(int)(turns >> 32) * 4.656612873077393e-10f, &s[p], &c[p]);  // 2^-31: half turns in [-1, 1]
+      }
+    }
+    long long row = tok;
+    bool keep = true;
+    if (a.rows) {
+      row = load_index(a.rows, a.rows_bits, tok);
+      keep = row >= 0 && row < a.out_rows;
+    }
+    if (lo < hq)
+      head_run<T, NORM, HALF>(a, a.seg[0], tok, tok, lo, min(hi, hq), sub, u, slots, o0, o1, rotated, c, s, gain[0]);
+    if (hi > hq && lo < hq + hk && (keep || !a.seg[1].scatter))
+      head_run<T, NORM, HALF>(a, a.seg[1], tok, a.seg[1].scatter ? row : tok, max(lo, hq) - hq, min(hi, hq + hk) - hq,
+                              sub, u, slots, o0, o1, rotated, c, s, gain[1]);
+    if (hi > hq + hk && (keep || !a.seg[2].scatter))
+      head_run<T, NORM, HALF>(a, a.seg[2], tok, a.seg[2].scatter ? row : tok, max(lo, hq + hk) - hq - hk,
+                              hi - hq - hk, sub, u, slots, o0, o1, rotated, c, s, gain[1]);
+  }
+}
+
+}  // namespace lbw
+
+using namespace lbw;
+
+// Checks one segment's pointers and strides; `elem` bytes per value.
+static int check_seg(const char* who, const char* name, const void* x, const void* out, long long xs_tok,
+                     long long xs_head, long long os_tok, long long os_head, int heads, int elem) {
+  if (!x || !out) return set_error(LBW_ERR_INVALID, "%s: null %s", who, name);
+  if (heads < 1 || heads > 1 << 20) return set_error(LBW_ERR_SHAPE, "%s: %d %s heads", who, heads, name);
+  const long long per = 16 / elem;
+  if (!aligned(x, 16) || !aligned(out, 16) || xs_tok % per || xs_head % per || os_tok % per || os_head % per)
+    return set_error(LBW_ERR_ALIGN, "%s: %s needs 16-byte aligned pointers and strides", who, name);
+  return LBW_OK;
+}
+
+static int check_common(const char* who, long long tokens, int head_dim, int dtype, const void* positions,
+                        int pos_bits, const lbw_rope_axes* rope) {
+  if (dtype != LBW_BF16 && dtype != LBW_FP16 && dtype != LBW_FP32)
+    return set_error(LBW_ERR_INVALID, "%s: dtype %d", who, dtype);
+  if (tokens < 0 || head_dim < 8 || head_dim % 8 || head_dim > 256)
+    return set_error(LBW_ERR_SHAPE, "%s: head_dim %d (a multiple of 8, at most 256)", who, head_dim);
+  if (!rope) return LBW_OK;
+  if (rope->pairs < 4 || rope->pairs % 4 || rope->pairs > 128 || 2 * rope->pairs > head_dim)
+    return set_error(LBW_ERR_SHAPE, "%s: %d rotated pairs of a %d-wide head (a multiple of 4, at most half of it)", who,
+                     rope->pairs, head_dim);
+  if (rope->axes < 1 || rope->axes > 8) return set_error(LBW_ERR_SHAPE, "%s: %d axes (1 to 8)", who, rope->axes);
+  for (int i = 0; i < rope->pairs; ++i)
+    if (rope->axis[i] >= rope->axes)
+      return set_error(LBW_ERR_INVALID, "%s: pair %d turns by axis %d of %d", who, i, rope->axis[i], rope->axes);
+  if (rope->layout != LBW_ROPE_INTERLEAVED && rope->layout != LBW_ROPE_HALF)
+    return set_error(LBW_ERR_INVALID, "%s: rope layout %d", who, rope->layout);
+  if (tokens > 0 && !positions) return set_error(LBW_ERR_INVALID, "%s: null positions", who);
+  if (pos_bits != 32 && pos_bits != 64) return set_error(LBW_ERR_INVALID, "%s: %d-bit positions", who, pos_bits);
+  return LBW_OK;
+}
+
+template <typename T, bool NORM>
+static void launch_t(const HeadArgs& a, unsigned blocks, cudaStream_t s) {
+  if (a.rope.layout == LBW_ROPE_HALF)
+    head_rope_kernel<T, NORM, true><<<blocks, hr::THREADS, 0, s>>>(a);
+  else
+    head_rope_kernel<T, NORM, false><<<blocks, hr::THREADS, 0, s>>>(a);
+}
+
+template <bool NORM>
+static int launch_head_rope(HeadArgs& a, int dtype, cudaStream_t s, const char* who) {
+  a.units = a.dim / 8;
+  a.group = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
+  const int total = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
+  a.chunk = total;
+  a.chunks = 1;
+  const long long items = a.tokens * a.chunks;
+  const long long want = (items + hr::THREADS / 32 - 1) / (hr::THREADS / 32);
+  const long long most = (long long)num_sms() * 8;
+  const unsigned blocks = (unsigned)(want < most ? want : most);
+  if (dtype == LBW_BF16)
+    launch_t<__nv_bfloat16, NORM>(a, blocks, s);
+  else if (dtype == LBW_FP16)
+    launch_t<__half, NORM>(a, blocks, s);
+  else
+    launch_t<float, NORM>(a, blocks, s);
+  return cuda_check(cudaGetLastError(), who);
+}
+
+extern "C" {
+
+int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, long long out_tok, long long out_head,
+                   long long tokens, int heads, int head_dim, int dtype, const void* positions, int pos_bits,
+                   long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream) {
+  const char* who = "axial_rope";
+  if (!rope) return set_error(LBW_ERR_INVALID, "%s: null rope", who);
+  int err = check_common(who, tokens, head_dim, dtype, positions, pos_bits, rope);
+  if (err) return err;
+  if (tokens == 0) return LBW_OK;
+  if ((err = check_seg(who, "x", x, out, x_tok, x_head, out_tok, out_head, heads, dtype == LBW_FP32 ? 4 : 2)))
+    return err;
+  HeadArgs a{};
+  a.seg[0] = HeadSeg{x, out, nullptr, x_tok, x_head, out_tok, out_head, heads, 0, 0, 0};
+  a.tokens = tokens;
+  a.dim = head_dim;
+  a.pos = positions;
+  a.pos_bits = pos_bits;
+  a.ps_tok = pos_tok;
+  a.ps_axis = pos_axis;
+  a.rope = *rope;
+  if (inverse)
+    for (int i = 0; i < a.rope.pairs; ++i) a.rope.step[i] = 0ull - a.rope.step[i];
+  return launch_head_rope<false>(a, dtype, reinterpret_cast<cudaStream_t>(stream), "axial_rope launch");
+}
+
+int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
+                         int head_dim, int dtype, float eps, const void* positions, int pos_bits, long long pos_tok,
+                         long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
+                         long long out_rows, void* stream) {
+  const char* who = "qk_headnorm_rope";
+  if (!q || !k) return set_error(LBW_ERR_INVALID, "%s: null q or k", who);
+  int err = check_common(who, tokens, head_dim, dtype, positions, pos_bits, rope);
+  if (err) return err;
+  if (!(eps >= 0.f)) return set_error(LBW_ERR_INVALID, "%s: eps %g", who, (double)eps);
+  if (k_rows && (k_rows_bits != 32 && k_rows_bits != 64))
+    return set_error(LBW_ERR_INVALID, "%s: %d-bit cache rows", who, k_rows_bits);
+  if (tokens == 0) return LBW_OK;
+  if (k_rows && out_rows < 0) return set_error(LBW_ERR_SHAPE, "%s: %lld cache rows", who, out_rows);
+  HeadArgs a{};
+  const lbw_head_rows* in[3] = {q, k, v};
+  const char* names[3] = {"q", "k", "v"};
+  for (int i = 0; i < 3; ++i) {
+    if (!in[i]) continue;
+    const lbw_head_rows& r = *in[i];
+    if ((err = check_seg(who, names[i], r.x, r.out, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads,
+                         dtype == LBW_FP32 ? 4 : 2)))
+      return err;
+    if (r.gamma && !aligned(r.gamma, r.gamma_f32 ? 4 : 2))
+      return set_error(LBW_ERR_ALIGN, "%s: gamma of %s is misaligned", who, names[i]);
+    a.seg[i] = HeadSeg{r.x,      r.out,   r.gamma,     r.x_tok, r.x_head, r.out_row,
+                       r.out_head, r.heads, r.gamma_f32, i == 2,  i > 0 && k_rows != nullptr};
+  }
+  a.tokens = tokens;
+  a.dim = head_dim;
+  a.eps = eps;
+  a.pos = positions;
+  a.pos_bits = pos_bits;
+  a.ps_tok = pos_tok;
+  a.ps_axis = pos_axis;
+  a.rows = k_rows;
+  a.rows_bits = k_rows_bits;
+  a.out_rows = out_rows;
+  if (rope) a.rope = *rope;
+  return launch_head_rope<true>(a, dtype, reinterpret_cast<cudaStream_t>(stream), "qk_headnorm_rope launch");
+}
+
+}  // extern "C"

@@ -40,6 +40,11 @@ inline int cuda_check(cudaError_t e, const char* what) {
 int make_tmap_2d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t rows,
                  uint64_t cols, uint64_t row_stride_elems, uint32_t box_cols, uint32_t box_rows);
 
+// Encodes a 3-D map of 16-bit elements [n2][n1][n0] (n0 contiguous; strides of n1 and n2 in elements), box
+// 64 x box1 x box2 with 128-byte swizzle. Out-of-bounds parts of a box are zero-filled.
+int make_tmap_3d(CUtensorMap* out, const void* base, CUtensorMapDataType dtype, uint64_t n0, uint64_t n1, uint64_t n2,
+                 uint64_t stride1, uint64_t stride2, uint32_t box1, uint32_t box2);
+
 int num_sms();
 // Row blocks (of 128) per tile group of the persistent GEMMs (see tile_coords): about 40 MB of activation rows
 // (K elements of elem_bytes each) so that a group stays in the 126 MB L2 with the weights streaming past.

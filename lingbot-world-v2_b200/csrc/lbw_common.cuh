@@ -115,6 +115,15 @@ LBW_DEV void tma_load_2d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0,
       "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
+LBW_DEV void tma_load_3d(void* dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+// Orders this thread's ordinary shared-memory writes before later reads of them by the tensor core or a bulk copy.
+LBW_DEV void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Plain bulk copy global -> shared (16-byte aligned addresses, size a multiple of 16).
 LBW_DEV void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -260,6 +269,10 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, int a_mn_major, 
          | ((uint32_t)b_mn_major << 16) // B major
          | ((uint32_t)(N >> 3) << 17)   // N
          | ((uint32_t)(M >> 4) << 24);  // M
+}
+// The same for f16 x f16 -> fp32 (A / B format 0).
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn_major, int b_mn_major) {
+  return idesc_bf16(M, N, a_mn_major, b_mn_major) & ~((1u << 7) | (1u << 10));
 }
 // Instruction descriptor, kind::mxf8f6f4 block-scaled: both operands E4M3 (fmt 0) or both E5M2 (fmt 1) with UE8M0
 // scales, K-major operands; sf_id selects the byte of the 32-bit TMEM scale column.

@@ -1,0 +1,83 @@
+// What the kernels of packed-sequence attention share: the description of a call, the lookup of a sequence in the
+// device arrays of starts and lengths, and the rounding of probabilities and outputs to the tensors' type.
+#pragma once
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "lbw_common.cuh"
+
+namespace lbw {
+
+struct PackedArgs {
+  const int* cu_q;    // [n_seqs + 1] first query row of each sequence
+  const int* cu_k;    // [n_seqs + 1] first key row
+  const int* k_lens;  // [n_seqs] keys in use, or null: all of the sequence's rows
+  int n_seqs;
+  int tq, tk;         // rows of q and of k / v: every start and length is clamped to them
+  int hq, hk, group;  // heads; group = hq / hk query heads share a kv head
+  int causal;
+  float scale_log2;
+  void* out;
+  long long os_tok, os_head;
+};
+
+struct PackedSeq {
+  int q0, nq, k0, nk;
+};
+
+// Sequence b of the call. The arrays live on the device, so nothing on the host has checked them: a start or length
+// that does not fit the tensors is cut to what does.
+LBW_DEV PackedSeq packed_seq(const PackedArgs& a, int b) {
+  PackedSeq s;
+  s.q0 = min(max(a.cu_q[b], 0), a.tq);
+  s.nq = min(max(a.cu_q[b + 1], s.q0), a.tq) - s.q0;
+  s.k0 = min(max(a.cu_k[b], 0), a.tk);
+  s.nk = min(max(a.cu_k[b + 1], s.k0), a.tk) - s.k0;
+  if (a.k_lens) s.nk = min(max(a.k_lens[b], 0), s.nk);
+  return s;
+}
+
+// Number of keys that query i of the sequence sees.
+LBW_DEV int packed_visible(const PackedArgs& a, const PackedSeq& s, int i) {
+  if (!a.causal) return s.nk;
+  const int n = i + 1 + s.nk - s.nq;
+  return n < 0 ? 0 : (n < s.nk ? n : s.nk);
+}
+
+// Whole warp: the sequence b and its local item l of global item w, where sequence b has count(b) items; false when w
+// lies past the last one. Each lane counts one sequence, 32 of them per step.
+template <typename F>
+LBW_DEV bool packed_find(int n_seqs, long long w, F count, int& b, long long& l) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int b0 = 0; b0 < n_seqs; b0 += 32) {
+    const long long own = b0 + lane < n_seqs ? (long long)count(b0 + lane) : 0;
+    long long upto = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > w);
+    if (hit) {
+      const int at = __ffs(hit) - 1;
+      b = b0 + at;
+      l = w - before - __shfl_sync(0xffffffffu, upto - own, at);
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
+}
+
+template <bool F16>
+LBW_DEV uint32_t pack_16(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    return pack_bf16(lo, hi);
+  }
+}
+
+}  // namespace lbw

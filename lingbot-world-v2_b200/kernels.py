@@ -4,13 +4,14 @@ Every wrapper validates dtypes/devices, passes raw pointers and the current CUDA
 non-zero status into ValueError / LbwError. Outputs may be passed in (written in place) or are
 allocated here.
 """
+import contextlib
 import ctypes
 import math
 
 import torch
 
 from . import _lib
-from ._lib import check, load, ptr, require_cuda, stream_of
+from ._lib import HeadRows, check, load, ptr, require_cuda, stream_of
 
 BF16 = torch.bfloat16
 HEAD_DIM = 128
@@ -733,4 +734,221 @@ def transpose_bf16(x, ldx, rows, cols, out, ldo):
     if _avail(x) < (rows - 1) * ldx + cols or _avail(out) < (cols - 1) * ldo + rows:
         raise ValueError("transpose_bf16: sizes")
     check(load().lbw_transpose_bf16(ptr(x), ldx, rows, cols, ptr(out), ldo, stream_of(x.device)), "transpose_bf16")
+    return out
+
+
+# ---- packed sequences: rotation by per-token positions, per-head q/k norm, attention --------------------------------
+
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # lbw_dtype (include/lbw.h)
+
+
+def _same_device(who, *tensors):
+    """The device of all the given tensors (None skipped); these operators have no gradient."""
+    require_cuda(*tensors)
+    given = [t for t in tensors if t is not None]
+    if any(t.device != given[0].device for t in given):
+        raise ValueError(f"{who}: tensors on different devices")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or with detached tensors")
+    return given[0].device
+
+
+def _on(device):
+    """Context in which `device` is the current one (the library launches on the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _heads3(who, name, t, dtype=None, dim=None):
+    """[tokens, heads, head_dim] view of a [tokens, heads, head_dim] or [1, tokens, heads, head_dim] tensor."""
+    if t.dim() == 4 and t.shape[0] == 1:
+        t = t[0]
+    if t.dim() != 3 or t.shape[1] < 1:
+        raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
+    if t.dtype != dtype and dtype is not None:
+        raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
+    if dim is not None and t.shape[2] != dim:
+        raise ValueError(f"{who}: head_dim of {name} is {t.shape[2]}, expected {dim}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{who}: {name} needs a contiguous head_dim")
+    return t
+
+
+def _writable(who, name, t):
+    """Refuses an output of which two elements share memory through a stride of zero."""
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{who}: {name} is an expanded tensor")
+    return t
+
+
+def _positions(who, positions, tokens, rope):
+    if positions.dim() == 1:
+        positions = positions[:, None]
+    if positions.dim() != 2 or positions.shape[0] != tokens or positions.shape[1] != rope.axes:
+        raise ValueError(f"{who}: positions must be [{tokens}, {rope.axes}], got {tuple(positions.shape)}")
+    return positions, _index_bits(who, "positions", positions)
+
+
+def _index_bits(who, name, t):
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{who}: {name} must be int32 or int64, got {t.dtype}")
+    return 32 if t.dtype == torch.int32 else 64
+
+
+def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
+    """x [tokens, heads, head_dim] (or [1, tokens, ...]; bf16, fp16 or fp32, strided) with every head rotated by
+    `rope` (rope.AxialRope) at the token's positions [tokens, axes] (int32 / int64, any values; [tokens] for one axis).
+    out: optional, x itself for in place. inverse=True undoes it; with positions that are differences it re-bases keys
+    that are already rotated."""
+    who = "axial_rope"
+    if _tracing(_eager):
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _op(who)(x, positions, list(rope.sections), rope.theta, rope.layout, rope.spectrum, list(rope.scale),
+                 bool(inverse), out)
+        return out
+    dev = _same_device(who, x, positions, out)
+    if x.dtype not in DTYPES:
+        raise ValueError(f"{who}: x is {x.dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
+    x3 = _heads3(who, "x", x)
+    tokens, heads, dim = x3.shape
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    o3 = _writable(who, "out", _heads3(who, "out", out, x.dtype, dim))
+    if o3.shape != x3.shape:
+        raise ValueError(f"{who}: out is {tuple(out.shape)}, x {tuple(x.shape)}")
+    pos, bits = _positions(who, positions, tokens, rope)
+    with _on(dev):
+        check(load().lbw_axial_rope(x3.data_ptr(), x3.stride(0), x3.stride(1), o3.data_ptr(), o3.stride(0),
+                                    o3.stride(1), tokens, heads, dim, DTYPES[x.dtype], pos.data_ptr(), bits,
+                                    pos.stride(0), pos.stride(1), rope.ref, int(bool(inverse)), stream_of(dev)),
+              who, launches=1 if tokens else 0)
+    return out
+
+
+def _head_rows(x, out, gamma):
+    return HeadRows(x.data_ptr(), out.data_ptr(), 0 if gamma is None else gamma.data_ptr(), x.stride(0), x.stride(1),
+                    out.stride(0), out.stride(1), x.shape[1], int(gamma is not None and gamma.dtype == torch.float32))
+
+
+def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_out=None, k_out=None, v=None,
+                     v_out=None, k_rows=None, _eager=False):
+    """RMSNorm of every head of q [tokens, hq, head_dim] and k [tokens, hk, head_dim] (bf16, fp16 or fp32; strided, so
+    slices of a fused q|k|v projection do), times gamma_q / gamma_k [head_dim] (the tensors' type or fp32; None: no
+    gain), then the rotation by `rope` (rope.AxialRope) at positions [tokens, axes], in one pass. Returns (q_out,
+    k_out). With k_rows [tokens] (int32 / int64, each row at most once) k goes to rows k_rows of the cache k_out
+    [rows, hk, head_dim], and v, copied, to the same rows of v_out; tokens whose row lies outside the cache (-1: padding)
+    write none. q_out may be q and, without k_rows, k_out may be k."""
+    who = "qk_headnorm_rope"
+    if _tracing(_eager):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        r = rope
+        _op(who)(q, k, gamma_q, gamma_k, float(eps), positions, list(r.sections) if r else [], r.theta if r else 1.0,
+                 r.layout if r else "", r.spectrum if r else "", list(r.scale) if r else [], q_out, k_out, v, v_out,
+                 k_rows)
+        return q_out, k_out
+    dev = _same_device(who, q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows)
+    if q.dtype not in DTYPES:
+        raise ValueError(f"{who}: q is {q.dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
+    q3 = _heads3(who, "q", q)
+    tokens, _, dim = q3.shape
+    k3 = _heads3(who, "k", k, q.dtype, dim)
+    if k3.shape[0] != tokens:
+        raise ValueError(f"{who}: {tokens} rows of q, {k3.shape[0]} of k")
+    for name, g in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
+        if g is not None and (g.shape != (dim,) or g.dtype not in (q.dtype, torch.float32) or not g.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be contiguous [{dim}] {q.dtype} or fp32, got {tuple(g.shape)} {g.dtype}")
+    if (positions is None) != (rope is None):
+        raise ValueError(f"{who}: give positions and rope, or neither")
+    if (v is None) != (v_out is None) or (v is not None and k_rows is None):
+        raise ValueError(f"{who}: v is copied to the rows k_rows of v_out: give all three, or no v")
+    if k_rows is not None and k_out is None:
+        raise ValueError(f"{who}: k_rows name rows of k_out: give it")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
+    qo = _writable(who, "q_out", _heads3(who, "q_out", q_out, q.dtype, dim))
+    ko = _writable(who, "k_out", _heads3(who, "k_out", k_out, q.dtype, dim))
+    if qo.shape != q3.shape or ko.shape[1] != k3.shape[1] or (k_rows is None and ko.shape[0] != tokens):
+        raise ValueError(f"{who}: q_out {tuple(q_out.shape)} / k_out {tuple(k_out.shape)} do not match q, k")
+    rows_bits, seg_v = 0, None
+    if k_rows is not None:
+        rows_bits = _index_bits(who, "k_rows", k_rows)
+        if k_rows.shape != (tokens,) or not k_rows.is_contiguous():
+            raise ValueError(f"{who}: k_rows must be contiguous [{tokens}], got {tuple(k_rows.shape)}")
+    if v is not None:
+        v3 = _heads3(who, "v", v, q.dtype, dim)
+        vo = _writable(who, "v_out", _heads3(who, "v_out", v_out, q.dtype, dim))
+        if v3.shape[0] != tokens or vo.shape[1] != v3.shape[1] or vo.shape[0] != ko.shape[0]:
+            raise ValueError(f"{who}: v {tuple(v.shape)} / v_out {tuple(v_out.shape)} do not match q and k_out")
+        seg_v = ctypes.byref(_head_rows(v3, vo, None))
+    pos, pos_bits, st0, st1 = None, 32, 0, 0
+    if rope is not None:
+        p2, pos_bits = _positions(who, positions, tokens, rope)
+        pos, st0, st1 = p2.data_ptr(), p2.stride(0), p2.stride(1)
+    with _on(dev):
+        check(load().lbw_qk_headnorm_rope(ctypes.byref(_head_rows(q3, qo, gamma_q)),
+                                          ctypes.byref(_head_rows(k3, ko, gamma_k)), seg_v, tokens, dim,
+                                          DTYPES[q.dtype], float(eps), pos, pos_bits, st0, st1,
+                                          rope.ref if rope is not None else None, ptr(k_rows), rows_bits, ko.shape[0],
+                                          stream_of(dev)), who, launches=1 if tokens else 0)
+    return q_out, k_out
+
+
+def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=None):
+    """Workspace (uint8) of packed_attention calls with these sizes, or None when they need none. Calls that may overlap
+    (other streams, graphs replayed side by side) need one each; packed_attention makes its own when given none."""
+    n = ctypes.c_longlong(0)
+    device = torch.device(device)
+    with torch.cuda.device(device):
+        check(load().lbw_packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0),
+                                                    ctypes.byref(n)), "packed_attention_workspace")
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+
+
+def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scale=None, out=None, max_q=None,
+                     workspace=None, _eager=False):
+    """Attention of a batch of sequences packed on one token axis: q [tq, hq, d], k / v [tk, hk, d] (bf16 or fp16, d 64
+    or 128, hq a multiple of hk; strided) -> out [tq, hq, d]. Sequence b: query rows cu_q[b]..cu_q[b + 1], key rows
+    cu_k[b]..cu_k[b + 1], of which the first k_lens[b] are in use if k_lens is given (a cache). causal: the last query
+    sees every key, the one before it one key less, and so on; a query that sees no key gets zeros. Rows of no sequence
+    are left as they are in `out`. cu_q, cu_k [n + 1] and k_lens [n] are int32 device tensors, read by the kernels (a
+    captured call follows what they hold at its replay). max_q: the most queries of a sequence, if known (speed only).
+    workspace: packed_attention_workspace(...) for callers that keep one; see there."""
+    who = "packed_attention"
+    if _tracing(_eager):
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
+        _op(who)(q, k, v, cu_q, cu_k, k_lens, bool(causal), float(scale), out, int(max_q or 0))
+        return out
+    dev = _same_device(who, q, k, v, cu_q, cu_k, k_lens, out, workspace)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"{who}: q is {q.dtype}, expected bf16 or fp16")
+    q3 = _heads3(who, "q", q)
+    tq, hq, dim = q3.shape
+    k3, v3 = _heads3(who, "k", k, q.dtype, dim), _heads3(who, "v", v, q.dtype, dim)
+    tk, hk = k3.shape[0], k3.shape[1]
+    if v3.shape != k3.shape:
+        raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
+    for name, t, want in (("cu_q", cu_q, n + 1), ("cu_k", cu_k, n + 1), ("k_lens", k_lens, n)):
+        if t is not None and (n < 0 or t.dtype != torch.int32 or t.shape != (want,) or not t.is_contiguous()):
+            raise ValueError(f"{who}: {name} must be contiguous int32 [{max(want, 0)}], got {tuple(t.shape)} {t.dtype}")
+    if max_q is not None and max_q < 0:
+        raise ValueError(f"{who}: max_q {max_q}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    o3 = _writable(who, "out", _heads3(who, "out", out, q.dtype, dim))
+    if o3.shape != q3.shape:
+        raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
+    scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
+    if workspace is None:
+        workspace = packed_attention_workspace(tq, tk, hq, hk, dim, n, dev, max_q)
+    with _on(dev):
+        check(load().lbw_packed_attention(
+            q3.data_ptr(), q3.stride(0), q3.stride(1), k3.data_ptr(), k3.stride(0), k3.stride(1), v3.data_ptr(),
+            v3.stride(0), v3.stride(1), o3.data_ptr(), o3.stride(0), o3.stride(1), cu_q.data_ptr(), cu_k.data_ptr(),
+            ptr(k_lens), n, tq, tk, hq, hk, dim, DTYPES[q.dtype], int(bool(causal)), scale, int(max_q or 0),
+            ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), stream_of(dev)),
+            who)
     return out

@@ -8,11 +8,13 @@ implementation that only describes its outputs, so the compiler traces the block
 runs the real kernels at execution. The torch wrappers of lbw_b200.kernels call these operators while a
 graph is being traced and the C ABI directly otherwise, so eager code pays no dispatcher cost.
 """
+import functools
 from typing import List, Optional
 
 import torch
 
 from . import kernels as K
+from .rope import AxialRope
 
 BF16 = torch.bfloat16
 
@@ -243,3 +245,52 @@ def _(a, a_s, w, w_s, bias, fmt):
 OPS = ("chunk_attention", "chunk_attention_partial", "chunk_attention_tail", "attention_merge", "layernorm_mod", "layernorm_mod_mx",
        "layernorm_affine_mx", "qkv_proj", "rmsnorm_rope", "qk_rmsnorm_rope", "linear_residual", "linear_rowss", "linear_gelu",
        "mx_linear_gelu", "mx_linear_residual", "mx_quantize_into", "mx_quantize", "mx_linear")
+
+
+@functools.lru_cache(None)
+def _axial(sections, theta, layout, spectrum, scale):
+    return AxialRope(sections, theta, layout, spectrum, scale)
+
+
+@torch.library.custom_op("lbw::axial_rope", mutates_args=("out",))
+def axial_rope(x: torch.Tensor, positions: torch.Tensor, sections: List[int], theta: float, layout: str, spectrum: str,
+               scale: List[float], inverse: bool, out: torch.Tensor) -> None:
+    """Rotation of every head by per-token positions (kernels.axial_rope)."""
+    K.axial_rope(x, positions, _axial(tuple(sections), theta, layout, spectrum, tuple(scale)), inverse=inverse, out=out,
+                 _eager=True)
+
+
+@axial_rope.register_fake
+def _(x, positions, sections, theta, layout, spectrum, scale, inverse, out):
+    return None
+
+
+@torch.library.custom_op("lbw::qk_headnorm_rope", mutates_args=("q_out", "k_out", "v_out"))
+def qk_headnorm_rope(q: torch.Tensor, k: torch.Tensor, gamma_q: Optional[torch.Tensor],
+                     gamma_k: Optional[torch.Tensor], eps: float, positions: Optional[torch.Tensor],
+                     sections: List[int], theta: float, layout: str, spectrum: str, scale: List[float],
+                     q_out: torch.Tensor, k_out: torch.Tensor, v: Optional[torch.Tensor],
+                     v_out: Optional[torch.Tensor], k_rows: Optional[torch.Tensor]) -> None:
+    """Per-head RMSNorm of q and k with the rotation, k and v to cache rows (kernels.qk_headnorm_rope)."""
+    rope = _axial(tuple(sections), theta, layout, spectrum, tuple(scale)) if sections else None
+    K.qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions, rope, q_out=q_out, k_out=k_out, v=v, v_out=v_out,
+                       k_rows=k_rows, _eager=True)
+
+
+@qk_headnorm_rope.register_fake
+def _(q, k, gamma_q, gamma_k, eps, positions, sections, theta, layout, spectrum, scale, q_out, k_out, v, v_out, k_rows):
+    return None
+
+
+@torch.library.custom_op("lbw::packed_attention", mutates_args=("out",))
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                     k_lens: Optional[torch.Tensor], causal: bool, scale: float, out: torch.Tensor,
+                     max_q: int) -> None:
+    """Attention of packed sequences (kernels.packed_attention)."""
+    K.packed_attention(q, k, v, cu_q, cu_k, k_lens=k_lens, causal=causal, softmax_scale=scale, out=out,
+                       max_q=max_q or None, _eager=True)
+
+
+@packed_attention.register_fake
+def _(q, k, v, cu_q, cu_k, k_lens, causal, scale, out, max_q):
+    return None

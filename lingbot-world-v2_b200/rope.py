@@ -9,6 +9,9 @@ freqs built at :3273-3278 from rope_params, wan/modules/model.py:47-53). Its gri
 are taken on the CPU in fp32 exactly as the reference does, so the tables are bit-identical to the
 reference grids' entries.
 """
+import ctypes
+import math
+
 import torch
 
 HEAD_DIM = 128
@@ -76,3 +79,56 @@ def _tables(freqs, f, h, w, start_frame, device):
     ang = torch.cat([fc[start_frame:start_frame + f, :s0].reshape(-1), fc[:h, s0:s0 + s1].reshape(-1),
                      fc[:w, s0 + s1:].reshape(-1)])
     return torch.cos(ang).to(device), torch.sin(ang).to(device)
+
+
+class RopeAxes(ctypes.Structure):
+    """lbw_rope_axes (include/lbw.h)."""
+    _fields_ = [("pairs", ctypes.c_int), ("axes", ctypes.c_int), ("layout", ctypes.c_int), ("reserved", ctypes.c_int),
+                ("axis", ctypes.c_ubyte * 128), ("step", ctypes.c_ulonglong * 128)]
+
+
+class AxialRope:
+    """Rotation of a head by integer positions on several axes, given per token (kernels.axial_rope,
+    kernels.qk_headnorm_rope): packed clips and images, each on a grid of its own.
+
+    sections   pairs turned by each axis, in order, e.g. (22, 21, 21) for (frame, height, width); their sum is a
+               multiple of 4 and at most half of the head; the head's dims beyond twice the sum stay as they are
+    theta      base of the angular frequencies
+    layout     "interleaved": pair i is dims (2i, 2i + 1); "half": dims (i, i + pairs)
+    spectrum   "axis": pair j of an axis with n pairs has theta^(-j / n), as rope_freqs does for each axis;
+               "head": pair i of all has theta^(-i / pairs), whichever axis turns it
+    scale      factor on an axis's positions (position interpolation), one number or one per axis
+
+    A model makes it once and keeps it; it holds no device memory.
+    """
+
+    LAYOUTS = {"interleaved": 0, "half": 1}
+
+    def __init__(self, sections, theta=10000.0, layout="interleaved", spectrum="axis", scale=1.0):
+        self.sections = tuple(int(n) for n in sections)
+        self.theta, self.layout, self.spectrum = float(theta), layout, spectrum
+        self.axes, self.pairs = len(self.sections), sum(self.sections)
+        self.scale = tuple(float(s) for s in scale) if isinstance(scale, (tuple, list)) else (float(scale),) * self.axes
+        if not 1 <= self.axes <= 8 or min(self.sections) < 0:
+            raise ValueError(f"AxialRope: sections {self.sections} (1 to 8 axes, no negative counts)")
+        if self.pairs < 4 or self.pairs % 4 or self.pairs > 128:
+            raise ValueError(f"AxialRope: {self.pairs} pairs (a multiple of 4, at most 128)")
+        if layout not in self.LAYOUTS:
+            raise ValueError(f"AxialRope: layout {layout!r} (one of {sorted(self.LAYOUTS)})")
+        if spectrum not in ("axis", "head"):
+            raise ValueError(f"AxialRope: spectrum {spectrum!r} ('axis' or 'head')")
+        if len(self.scale) != self.axes or not all(math.isfinite(s) for s in self.scale):
+            raise ValueError(f"AxialRope: scale {scale!r} needs one finite value per axis")
+        if not (math.isfinite(self.theta) and self.theta > 0):
+            raise ValueError(f"AxialRope: theta {theta!r}")
+        self.axis_of_pair = [a for a, n in enumerate(self.sections) for _ in range(n)]
+        self.inv_freq = []                                   # radians per position, 64 bits
+        for a, n in enumerate(self.sections):
+            for j in range(n):
+                e = j / n if spectrum == "axis" else len(self.inv_freq) / self.pairs
+                self.inv_freq.append(self.scale[a] * self.theta ** -e)
+        self.c = RopeAxes(self.pairs, self.axes, self.LAYOUTS[layout], 0)
+        for i, f in enumerate(self.inv_freq):
+            self.c.axis[i] = self.axis_of_pair[i]
+            self.c.step[i] = round(f / (2 * math.pi) * 2.0 ** 64) % (1 << 64)
+        self.ref = ctypes.byref(self.c)

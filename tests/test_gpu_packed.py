@@ -1,0 +1,448 @@
+"""Packed-sequence operators on a B200 against their 64-bit forms, every value within its own bound (packed_oracle)."""
+import pytest
+import torch
+
+import packed_oracle as po
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def _randn(dev, seed, *shape, dtype=BF, scale=1.0):
+    return (torch.randn(*shape, generator=_gen(dev, seed), device=dev) * scale).to(dtype)
+
+
+def _cu(lens, dev):
+    return torch.tensor([0] + list(lens), dtype=torch.int64).cumsum(0).to(torch.int32).to(dev)
+
+
+# ---- rotation -----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("tokens,heads,dim,sections", [(1, 1, 8, (4,)), (7, 3, 64, (16, 16)), (300, 5, 80, (20, 10, 10)),
+                                                       (33, 40, 128, (22, 21, 21)), (5, 7, 256, (60, 4, 0, 64)),
+                                                       (64, 2, 96, (12,)), (9, 33, 128, (64,))])
+def test_axial_rope(cuda_dev, dtype, layout, tokens, heads, dim, sections):
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    r = AxialRope(sections, layout=layout, spectrum="head" if heads == 7 else "axis", scale=0.25 if heads == 5 else 1.0)
+    x = _randn(cuda_dev, tokens + dim, tokens, heads, dim, dtype=dtype)
+    pos = torch.randint(-3000, 3000, (tokens, len(sections)), generator=_gen(cuda_dev, 1), device=cuda_dev)
+    if heads != 3:
+        pos = pos.to(torch.int32)
+    y, size = po.rotate(x.double(), pos, r)
+    bound = po.head_bound(y, size, dtype, dim, False)
+    out = K.axial_rope(x, pos, r)
+    assert po.within(out, y, bound) <= 1
+    assert torch.equal(out[..., 2 * sum(sections):], x[..., 2 * sum(sections):])
+    yi, size = po.rotate(x.double(), pos, r, inverse=True)
+    keep = x.clone()
+    assert K.axial_rope(keep, pos, r, inverse=True, out=keep) is keep
+    assert po.within(keep, yi, po.head_bound(yi, size, dtype, dim, False)) <= 1
+
+
+def test_axial_rope_far_positions_strides_and_specials(cuda_dev):
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    r = AxialRope((32, 32))
+    far = torch.tensor([[0, 1], [2 ** 31 - 1, -2 ** 31], [10 ** 6, 10 ** 7], [2 ** 40 + 12345, -2 ** 50]],
+                       device=cuda_dev)
+    wide = _randn(cuda_dev, 2, 4, 9, 256, dtype=F32)
+    x = wide[:, 1::2, 64:192]                                             # every second head, inner dims
+    y, size = po.rotate(x.double(), far, r)
+    dst = torch.full((4, 4, 136), 7.0, device=cuda_dev)
+    K.axial_rope(x, far.t().contiguous().t(), r, out=dst[..., :128])      # positions with swapped strides
+    assert po.within(dst[..., :128], y, po.head_bound(y, size, F32, 128, False)) <= 1
+    assert bool((dst[..., 128:] == 7).all())
+    x = _randn(cuda_dev, 3, 3, 2, 96, dtype=BF)
+    x[0, 0, 95], x[1, 1, 90] = float("inf"), float("nan")                 # in the dims that pass through
+    out = K.axial_rope(x, torch.arange(3, device=cuda_dev), AxialRope((40,)))
+    assert torch.equal(out[..., 80:].view(torch.int16), x[..., 80:].view(torch.int16))
+    assert torch.isfinite(out[..., :80].float()).all()
+    zero = torch.zeros(3, 1, dtype=torch.int32, device=cuda_dev)
+    assert torch.equal(K.axial_rope(x[..., :80], zero, AxialRope((40,))), x[..., :80])
+
+
+# ---- per-head norm + rotation -------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("tokens,hq,hk,dim,sections,layout", [
+    (1, 1, 1, 64, (32,), "half"), (5, 12, 12, 128, (22, 21, 21), "interleaved"), (37, 7, 1, 80, (20, 20), "half"),
+    (400, 8, 2, 96, (10, 10, 12), "interleaved"), (3, 40, 8, 128, (64,), "half"), (11, 3, 3, 256, (64, 32), "half"),
+    (2000, 4, 2, 16, (4,), "interleaved"), (6, 5, 5, 128, None, "interleaved")])
+def test_qk_headnorm_rope(cuda_dev, dtype, tokens, hq, hk, dim, sections, layout):
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    rope = AxialRope(sections, layout=layout) if sections else None
+    qkv = _randn(cuda_dev, tokens + hq, tokens, hq + 2 * hk, dim, dtype=dtype, scale=2.0)
+    qkv[0, 0] = 0                                                          # a head of zeros stays zeros
+    q, k = qkv[:, :hq], qkv[:, hq:hq + hk]
+    gq = _randn(cuda_dev, 3, dim, dtype=dtype)
+    gk = None if hq == 7 else _randn(cuda_dev, 4, dim, dtype=F32)
+    pos = torch.randint(0, 90000, (tokens, len(sections)), generator=_gen(cuda_dev, 5), device=cuda_dev) if sections else None
+    before = qkv.clone()
+    qo, ko = K.qk_headnorm_rope(q, k, gq, gk, 1e-6, pos, rope)
+    assert torch.equal(qkv, before)
+    for got, x, g in ((qo, q, gq), (ko, k, gk)):
+        n = po.norm(x, g, 1e-6)
+        y, size = po.rotate(n, pos, rope) if rope else (n, n.abs())
+        assert po.within(got, y, po.head_bound(y, size, dtype, dim, True)) <= 1
+    assert bool((qo[0, 0] == 0).all())
+    K.qk_headnorm_rope(q, k, gq, gk, 1e-6, pos, rope, q_out=q, k_out=k)     # in place, inside the fused tensor
+    assert torch.equal(q, qo) and torch.equal(k, ko) and torch.equal(qkv[:, hq + hk:], before[:, hq + hk:])
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tokens,hq,hk,dim", [(1, 8, 2, 128), (9, 3, 3, 64), (130, 32, 8, 128), (20, 1, 5, 80)])
+def test_qk_headnorm_rope_writes_cache_rows(cuda_dev, index, tokens, hq, hk, dim):
+    """Rows in any order; padding (-1) and rows past the cache are not written; every other row stays."""
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    rope = AxialRope((dim // 2,), layout="half")
+    qkv = _randn(cuda_dev, 1, tokens, hq + 2 * hk, dim)
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    pos = torch.arange(tokens, device=cuda_dev, dtype=torch.int32) + 100
+    cap = tokens * 2 + 3
+    rows = torch.randperm(cap, generator=torch.Generator().manual_seed(2))[:tokens]
+    rows[tokens // 2] = -1
+    if tokens > 5:
+        rows[5], rows[3] = cap, -2 ** 31
+    rows = rows.to(index).to(cuda_dev)
+    kc, vc = (torch.full((cap, hk, 2 * dim), 9.0, dtype=BF, device=cuda_dev)[..., :dim] for _ in range(2))
+    want_k, want_v = kc.clone(), vc.clone()
+    qo, ko = K.qk_headnorm_rope(q, k, None, None, 1e-5, pos, rope)
+    keep = (rows >= 0) & (rows < cap)
+    want_k[rows[keep].long()], want_v[rows[keep].long()] = ko[keep], v[keep]
+    got_q, got_k = K.qk_headnorm_rope(q, k, None, None, 1e-5, pos, rope, k_out=kc, v=v, v_out=vc, k_rows=rows)
+    assert torch.equal(got_q, qo) and got_k is kc
+    assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
+
+
+def test_head_operators_refuse(cuda_dev):
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    r = AxialRope((32,))
+    x = torch.zeros(4, 2, 64, dtype=BF, device=cuda_dev)
+    pos = torch.zeros(4, dtype=torch.int32, device=cuda_dev)
+    g = torch.ones(64, dtype=BF, device=cuda_dev)
+    bad = [
+        lambda: K.axial_rope(x.double(), pos, r), lambda: K.axial_rope(x[..., ::2], pos, r),
+        lambda: K.axial_rope(x, pos[:3], r), lambda: K.axial_rope(x, pos.float(), r),
+        lambda: K.axial_rope(x, pos, AxialRope((8, 8))), lambda: K.axial_rope(x[..., :56], pos, r),
+        lambda: K.axial_rope(x, pos, r, out=x[:1].expand(4, 2, 64)), lambda: K.axial_rope(x, pos.cpu(), r),
+        lambda: K.axial_rope(x[..., 4:], pos, AxialRope((28,))),            # 60 wide
+        lambda: K.axial_rope(torch.zeros(4, 2, 68, dtype=BF, device=cuda_dev)[..., :64], pos, r),   # stride 68
+        lambda: K.axial_rope(x.clone().requires_grad_(), pos, r),
+        lambda: K.qk_headnorm_rope(x, x[:3], g, g, 1e-6, pos, r), lambda: K.qk_headnorm_rope(x, x, g[:32], g, 1e-6, pos, r),
+        lambda: K.qk_headnorm_rope(x, x, g.half(), g, 1e-6, pos, r), lambda: K.qk_headnorm_rope(x, x.half(), g, g, 1e-6, pos, r),
+        lambda: K.qk_headnorm_rope(x, x, g, g, 1e-6, pos), lambda: K.qk_headnorm_rope(x, x, g, g, -1.0, pos, r),
+        lambda: K.qk_headnorm_rope(x, x, g, g, 1e-6, pos, r, v=x, v_out=x),
+        lambda: K.qk_headnorm_rope(x, x, g, g, 1e-6, pos, r, k_rows=pos),
+        lambda: K.qk_headnorm_rope(x, x, g, g, 1e-6, pos, r, k_out=x.clone(), k_rows=pos[:2]),
+        lambda: K.qk_headnorm_rope(x, x, g, g, 1e-6, pos, r, k_out=x.clone(), k_rows=pos, v=x, v_out=x[:2].clone())]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    assert K.axial_rope(x[:0], pos[:0], r).shape == (0, 2, 64)
+    qo, ko = K.qk_headnorm_rope(x[:0], x[:0], g, g, 1e-6, pos[:0], r)
+    assert qo.shape == ko.shape == (0, 2, 64)
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------
+
+
+def _attention_case(dev, seed, q_lens, k_lens, hq, hk, dim, dtype, qk_scale=1.5):
+    q = _randn(dev, seed, sum(q_lens), hq, dim, dtype=dtype, scale=qk_scale)
+    k = _randn(dev, seed + 1, sum(k_lens), hk, dim, dtype=dtype)
+    v = _randn(dev, seed + 2, sum(k_lens), hk, dim, dtype=dtype)
+    return q, k, v, _cu(q_lens, dev), _cu(k_lens, dev)
+
+
+LENGTHS = [
+    ([1], [1]), ([128], [128]), ([129], [129]), ([257], [257]), ([64, 1, 200], [64, 1, 200]), ([3, 0, 5], [3, 0, 5]),
+    ([700], [700]), ([1, 1, 1], [300, 1, 77]), ([5, 130], [400, 131]), ([200, 40], [100, 0]), ([0, 0], [10, 3]),
+    (list(range(1, 70)), list(range(1, 70))), ([2, 260], [1000, 1300]), ([16, 17], [129, 127]),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 2), (6, 2), (8, 1), (10, 2), (14, 2), (34, 2)])
+@pytest.mark.parametrize("lens", LENGTHS, ids=lambda v: "-".join(map(str, v[0][:4])) + "_" + "-".join(map(str, v[1][:4])))
+def test_packed_attention(cuda_dev, lens, heads, causal):
+    import lbw_b200._lib as L
+    import lbw_b200.kernels as K
+    dim, dtype = (64, 128)[len(lens[0]) % 2], (BF, HF)[sum(lens[0]) % 2]
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 7, *lens, *heads, dim, dtype)
+    want, bound = po.attention(q, k, v, cu_q, cu_k, causal=causal)
+    for max_q in (None, max(lens[0])):
+        out = K.packed_attention(q, k, v, cu_q, cu_k, causal=causal, max_q=max_q)
+        assert po.within(out, want, bound) <= 1
+    L.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_attention_long(cuda_dev, dtype, dim, causal):
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 3, [2500, 900], [2500, 1777], 6, 2, dim, dtype, qk_scale=3.0)
+    want, bound = po.attention(q, k, v, cu_q, cu_k, causal=causal, scale=0.2)
+    out = K.packed_attention(q, k, v, cu_q, cu_k, causal=causal, softmax_scale=0.2)
+    assert po.within(out, want, bound) <= 1
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 3, 9, 40])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 2), (5, 1), (32, 1)])
+def test_packed_attention_over_a_cache(cuda_dev, dtype, dim, q_len, heads):
+    """Slabs with room to spare; what lies past a sequence's length is NaN and must not matter."""
+    import lbw_b200.kernels as K
+    lens, cap = [5000, q_len, 129, 1023, 0, 128], 5001
+    hq, hk = heads
+    n = len(lens)
+    q = _randn(cuda_dev, 1, n * q_len, hq, dim, dtype=dtype)
+    k, v = (torch.full((n * cap, hk, dim), float("nan"), dtype=dtype, device=cuda_dev) for _ in range(2))
+    for b, m in enumerate(lens):
+        k[b * cap:b * cap + m] = _randn(cuda_dev, 10 + b, m, hk, dim, dtype=dtype)
+        v[b * cap:b * cap + m] = _randn(cuda_dev, 20 + b, m, hk, dim, dtype=dtype)
+    cu_q, cu_k = _cu([q_len] * n, cuda_dev), _cu([cap] * n, cuda_dev)
+    k_lens = torch.tensor(lens, dtype=torch.int32, device=cuda_dev)
+    want, bound = po.attention(q, k, v, cu_q, cu_k, k_lens)
+    for max_q in (None, q_len):
+        out = K.packed_attention(q, k, v, cu_q, cu_k, k_lens=k_lens, max_q=max_q)
+        assert po.within(out, want, bound) <= 1
+
+
+def test_packed_attention_mixed_batch_and_rows_behind(cuda_dev):
+    """Prompts and single tokens in one call; query rows of no sequence keep what they held; strided tensors."""
+    import lbw_b200.kernels as K
+    hq, hk, d = 8, 2, 128
+    q_lens, k_lens = [300, 1, 1, 17, 2, 0, 129], [300, 2000, 5, 40, 2, 9, 4000]
+    qkv = _randn(cuda_dev, 1, sum(q_lens) + 30, hq + 2, d)
+    q = qkv[:, 1:hq + 1]
+    kv = _randn(cuda_dev, 2, 2, hk, sum(k_lens) + 50, d)                   # head-major keys and values
+    k, v = kv[0].transpose(0, 1), kv[1].transpose(0, 1)
+    v[sum(k_lens):] = float("nan")
+    cu_q, cu_k = _cu(q_lens, cuda_dev) + 4, _cu(k_lens, cuda_dev)           # the first rows belong to nobody either
+    buf = torch.full((q.shape[0], 2 * hq, d), 5.0, dtype=BF, device=cuda_dev)
+    out = buf[:, ::2]
+    want, bound = po.attention(q, k, v, cu_q, cu_k)
+    K.packed_attention(q, k, v, cu_q, cu_k, out=out)
+    rows = slice(4, 4 + sum(q_lens))
+    assert po.within(out[rows], want[rows], bound[rows]) <= 1
+    assert bool((out[:4] == 5).all()) and bool((out[4 + sum(q_lens):] == 5).all()) and bool((buf[:, 1::2] == 5).all())
+
+
+def test_packed_attention_peaked_and_huge_scores(cuda_dev):
+    """Scores far from zero (the running maximum moves by thousands), and one key that takes everything."""
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, [300, 1], [900, 700], 4, 2, 128, BF)
+    k[::37] *= 40
+    q *= 4
+    want, bound = po.attention(q, k, v, cu_q, cu_k)
+    assert po.within(K.packed_attention(q, k, v, cu_q, cu_k), want, bound) <= 1
+    k[:] = -60.0
+    q[:] = 60.0                                                            # every score the same: -40,729
+    want, bound = po.attention(q, k, v, cu_q, cu_k)
+    assert po.within(K.packed_attention(q, k, v, cu_q, cu_k), want, bound) <= 1
+
+
+def test_packed_attention_nan_stays_with_its_sequence(cuda_dev):
+    """A NaN key or value reaches every row that sees it and no other sequence; NaN keys ahead of a row do not."""
+    import lbw_b200.kernels as K
+    for lens in ([130, 200, 60], [1, 1, 1]):
+        ks = [130, 200, 60]
+        q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, lens, ks, 4, 2, 128, BF)
+        clean = K.packed_attention(q, k, v, cu_q, cu_k)
+        k[130 + 150] = float("nan")
+        out = K.packed_attention(q, k, v, cu_q, cu_k)
+        first = sum(lens[:2]) - 50 if lens[1] > 1 else 1                    # first query that sees key 150
+        last = sum(lens[:2])
+        assert torch.isnan(out[first:last].float()).all()
+        assert torch.equal(out[:first], clean[:first]) and torch.equal(out[last:], clean[last:])
+        k, v = k.nan_to_num(0.5), v.clone()
+        v[130 + 3] = float("inf")
+        out = K.packed_attention(q, k, v, cu_q, cu_k)
+        assert torch.isfinite(out[:lens[0]].float()).all() and torch.isfinite(out[last:].float()).all()
+
+
+def test_packed_attention_bad_starts_stay_inside(cuda_dev):
+    """Starts and lengths that do not fit are cut to the tensors: no row of another sequence is lost, none invented."""
+    import lbw_b200._lib as L
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, [40, 40], [40, 40], 4, 2, 64, BF)
+    want, bound = po.attention(q, k, v, cu_q, cu_k, causal=False)
+    big = torch.tensor([1 << 30, 40], dtype=torch.int32, device=cuda_dev)
+    out = K.packed_attention(q, k, v, cu_q, cu_k, k_lens=big, causal=False)
+    assert po.within(out, want, bound) <= 1
+    far_q = torch.tensor([0, 40, 1 << 30], dtype=torch.int32, device=cuda_dev)
+    far_k = torch.tensor([-7, 40, 1 << 30], dtype=torch.int32, device=cuda_dev)
+    out = K.packed_attention(q, k, v, far_q, far_k, causal=False)
+    assert po.within(out, want, bound) <= 1
+    low = torch.tensor([-5, 0], dtype=torch.int32, device=cuda_dev)
+    out = K.packed_attention(q, k, v, cu_q, cu_k, k_lens=low, causal=False)
+    assert bool((out == 0).all())
+    L.check_device_status()
+
+
+def test_packed_attention_offsets_past_32_bits(cuda_dev):
+    """Keys whose element offset is beyond 2^32: a cache of 34 million rows, of which the last are used."""
+    import lbw_b200.kernels as K
+    rows, d = (1 << 25) + 3000, 128
+    k, v = (torch.empty(rows, 1, d, dtype=BF, device=cuda_dev) for _ in range(2))
+    k[-3000:], v[-3000:] = _randn(cuda_dev, 1, 3000, 1, d), _randn(cuda_dev, 2, 3000, 1, d)
+    q = _randn(cuda_dev, 3, 21, 2, d)
+    start = rows - 3000
+    cu_k = torch.tensor([start, start + 1000, rows], dtype=torch.int32, device=cuda_dev)
+    for q_lens in ([1, 20], [1, 1]):
+        cu_q = _cu(q_lens, cuda_dev)
+        want, bound = po.attention(q, k[start:], v[start:], cu_q, cu_k - start)
+        out = K.packed_attention(q, k, v, cu_q, cu_k)
+        n = sum(q_lens)
+        assert po.within(out[:n], want[:n], bound[:n]) <= 1
+
+
+def test_packed_attention_refuses(cuda_dev):
+    import lbw_b200.kernels as K
+    x = torch.zeros(4, 2, 64, dtype=BF, device=cuda_dev)
+    cu = _cu([4], cuda_dev)
+    bad = [
+        lambda: K.packed_attention(x.float(), x.float(), x.float(), cu, cu), lambda: K.packed_attention(x, x.half(), x, cu, cu),
+        lambda: K.packed_attention(x, x, x[:3], cu, cu), lambda: K.packed_attention(x[:, :1], x, x, cu, cu),
+        lambda: K.packed_attention(x[..., :32], x[..., :32], x[..., :32], cu, cu),
+        lambda: K.packed_attention(x, x, x, cu.long(), cu), lambda: K.packed_attention(x, x, x, cu, cu[:1]),
+        lambda: K.packed_attention(x, x, x, cu, cu, k_lens=cu), lambda: K.packed_attention(x, x, x, cu, cu.cpu()),
+        lambda: K.packed_attention(x, x, x, cu, cu, softmax_scale=-1.0), lambda: K.packed_attention(x, x, x, cu, cu, max_q=-1),
+        lambda: K.packed_attention(x, x[:1].expand(4, 2, 64), x, cu, cu),
+        lambda: K.packed_attention(x, x, x, cu, cu, out=x[:, :1].expand(4, 2, 64)),
+        lambda: K.packed_attention(x.clone().requires_grad_(), x, x, cu, cu),
+        lambda: K.packed_attention(torch.zeros(4, 2, 68, dtype=BF, device=cuda_dev)[..., 2:66], x, x, cu, cu)]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    assert K.packed_attention(x[:0], x, x, cu * 0, cu).shape == (0, 2, 64)
+    none = torch.full_like(x, 3.0)
+    K.packed_attention(x, x, x, cu[:1], cu[:1], out=none)                   # no sequences: nothing is written
+    assert bool((none == 3).all())
+    assert bool((K.packed_attention(x, x[:0], x[:0], cu, cu * 0) == 0).all())
+
+
+# ---- together -----------------------------------------------------------------------------------------------------
+
+
+def _layer(K, rope, qkv, hq, hk, gq, gk, pos, rows, kc, vc, cu_q, cu_k, k_lens, out=None, max_q=None):
+    q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    qo, _ = K.qk_headnorm_rope(q, k, gq, gk, 1e-6, pos, rope, k_out=kc, v=v, v_out=vc, k_rows=rows)
+    return K.packed_attention(qo, kc, vc, cu_q, cu_k, k_lens=k_lens, out=out, max_q=max_q)
+
+
+def test_prompt_then_tokens_over_the_cache(cuda_dev):
+    """A serving loop: two prompts fill their cache slabs, then single tokens; each step against 64 bits over the
+    rounded q, k, v that it really has."""
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    hq, hk, d, cap, lens = 8, 2, 128, 400, [300, 77]
+    rope = AxialRope((22, 21, 21))
+    gq, gk = _randn(cuda_dev, 1, d), _randn(cuda_dev, 2, d)
+    kc, vc = (torch.full((2 * cap, hk, d), float("nan"), dtype=BF, device=cuda_dev) for _ in range(2))
+    cu_k = _cu([cap, cap], cuda_dev)
+    done = [0, 0]
+    for step, new in enumerate((lens, [1, 1], [1, 1], [5, 1], [0, 1])):
+        qkv = _randn(cuda_dev, 50 + step, sum(new), hq + 2 * hk, d)
+        at = torch.cat([torch.arange(done[b], done[b] + new[b]) for b in range(2)])
+        seq = torch.repeat_interleave(torch.arange(2), torch.tensor(new))
+        pos = torch.stack([at // 50, at // 10 % 5, at % 10], 1).to(cuda_dev)
+        rows = (at + seq * cap).to(cuda_dev)
+        done = [a + n for a, n in zip(done, new)]
+        k_lens = torch.tensor(done, dtype=torch.int32, device=cuda_dev)
+        cu_q = _cu(new, cuda_dev)
+        out = _layer(K, rope, qkv, hq, hk, gq, gk, pos, rows, kc, vc, cu_q, cu_k, k_lens)
+        qn, size = po.rotate(po.norm(qkv[:, :hq], gq, 1e-6), pos, rope)
+        kn, ksize = po.rotate(po.norm(qkv[:, hq:hq + hk], gk, 1e-6), pos, rope)
+        q16, _ = K.qk_headnorm_rope(qkv[:, :hq], qkv[:, hq:hq + hk], gq, gk, 1e-6, pos, rope)
+        assert po.within(q16, qn, po.head_bound(qn, size, BF, d, True)) <= 1
+        assert po.within(kc[rows], kn, po.head_bound(kn, ksize, BF, d, True)) <= 1
+        assert torch.equal(vc[rows], qkv[:, hq + hk:])
+        want, bound = po.attention(q16, kc, vc, cu_q, cu_k, k_lens)
+        assert po.within(out, want, bound) <= 1
+
+
+def test_captured_step_follows_new_lengths_and_rows(cuda_dev):
+    """One graph of the norm + cache write + attention, replayed with other lengths, rows and a padded batch entry."""
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    hq, hk, d, cap, n = 8, 2, 64, 600, 5
+    rope = AxialRope((32,), layout="half")
+    kc, vc = (_randn(cuda_dev, s, n * cap, hk, d) for s in (1, 2))
+    qkv = _randn(cuda_dev, 3, n, hq + 2 * hk, d)
+    pos, rows = (torch.zeros(n, dtype=torch.int64, device=cuda_dev) for _ in range(2))
+    k_lens = torch.zeros(n, dtype=torch.int32, device=cuda_dev)
+    cu_q, cu_k = _cu([1] * n, cuda_dev), _cu([cap] * n, cuda_dev)
+    out = torch.empty(n, hq, d, dtype=BF, device=cuda_dev)
+
+    def step():
+        return _layer(K, rope, qkv, hq, hk, None, None, pos, rows, kc, vc, cu_q, cu_k, k_lens, out=out, max_q=1)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for lens in ([600, 1, 300, 129, 0], [1, 599, 2, 256, 77]):
+        at = torch.tensor(lens) - 1
+        pos.copy_(at)
+        rows.copy_(torch.where(at < 0, at, at + torch.arange(n) * cap))
+        k_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        qkv.copy_(_randn(cuda_dev, sum(lens), n, hq + 2 * hk, d))
+        before = kc.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        q16, k16 = K.qk_headnorm_rope(qkv[:, :hq], qkv[:, hq:hq + hk], None, None, 1e-6, pos, rope)
+        used = rows[rows >= 0]
+        before[used] = k16[rows >= 0]
+        assert torch.equal(kc, before)
+        want, bound = po.attention(q16, kc, vc, cu_q, cu_k, k_lens)
+        assert po.within(out, want, bound) <= 1
+
+
+def test_two_streams_at_once(cuda_dev):
+    import lbw_b200.kernels as K
+    cases = [_attention_case(cuda_dev, s, [1, 1], [5000, 300 + s], 8, 2, 128, BF) for s in (1, 40)]
+    cases += [_attention_case(cuda_dev, s, [130, 60], [2130, 60 + s], 8, 2, 128, BF) for s in (2, 41)]
+    want = [K.packed_attention(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[] for _ in cases]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(K.packed_attention(*c))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+
+
+def test_compiled_graph_equals_eager(cuda_dev):
+    import lbw_b200.kernels as K
+    import lbw_b200.ops  # noqa: F401
+    from lbw_b200.rope import AxialRope
+    rope = AxialRope((16, 16), layout="half")
+    qkv = _randn(cuda_dev, 1, 50, 6, 64)
+    pos = torch.arange(100, device=cuda_dev).view(50, 2)
+    cu = _cu([20, 30], cuda_dev)
+
+    def f(qkv, pos, cu):
+        q, k = K.qk_headnorm_rope(qkv[:, :2], qkv[:, 2:4], None, None, 1e-6, pos, rope)
+        return K.packed_attention(K.axial_rope(q, pos, rope), k, qkv[:, 4:], cu, cu)
+
+    assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(qkv, pos, cu), f(qkv, pos, cu))

@@ -1,0 +1,129 @@
+"""Packed-sequence operators without a GPU: the rotation's description, refusals, and the C entries' argument checks."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import lbw_b200._lib as L
+import lbw_b200.kernels as K
+import lbw_b200.rope as rope
+
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import __graft_entry__
+    __graft_entry__.build()
+    return L.load()
+
+
+def test_axial_rope_frequencies_are_the_three_axis_tables():
+    r = rope.AxialRope((22, 21, 21))
+    freqs = rope.rope_freqs(max_frames=2)[1].double()          # angles at position 1
+    assert torch.allclose(torch.tensor(r.inv_freq, dtype=torch.float64), freqs, rtol=1e-6)
+    assert r.axis_of_pair == [0] * 22 + [1] * 21 + [2] * 21
+    for i, f in enumerate(r.inv_freq):
+        assert abs(r.c.step[i] / 2.0 ** 64 * 2 * math.pi - f) <= f * 2.0 ** -52 + 2.0 ** -64 * 7
+
+
+def test_axial_rope_head_spectrum_and_scale():
+    r = rope.AxialRope((3, 5), theta=100.0, spectrum="head", layout="half", scale=(0.5, 2.0))
+    want = [100.0 ** (-i / 8) * (0.5 if i < 3 else 2.0) for i in range(8)]
+    assert r.inv_freq == pytest.approx(want, rel=1e-15)
+    assert (r.c.pairs, r.c.axes, r.c.layout) == (8, 2, 1)
+
+
+@pytest.mark.parametrize("kw", [dict(sections=()), dict(sections=(3,)), dict(sections=(5, -1)), dict(sections=(132,)),
+                                dict(sections=(8,), layout="pairs"), dict(sections=(8,), spectrum="x"),
+                                dict(sections=(8,), scale=(1.0, 1.0)), dict(sections=(8,), scale=math.inf),
+                                dict(sections=(8,), theta=0.0), dict(sections=(4,) * 9)])
+def test_axial_rope_refuses(kw):
+    with pytest.raises(ValueError):
+        rope.AxialRope(**kw)
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(4, 2, 64, dtype=BF)
+    pos = torch.zeros(4, 1, dtype=torch.int32)
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    r = rope.AxialRope((32,))
+    for call in (lambda: K.axial_rope(x, pos, r), lambda: K.qk_headnorm_rope(x, x, None, None, 1e-6, pos, r),
+                 lambda: K.packed_attention(x, x, x, cu, cu)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def _rope(pairs=32, axes=1, layout=0, axis=0):
+    r = rope.RopeAxes(pairs, axes, layout, 0)
+    r.axis[0] = axis
+    return ctypes.byref(r)
+
+
+P = ctypes.c_void_p(4096)
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(x=None), L.LBW_ERR_INVALID), (dict(out=None), L.LBW_ERR_INVALID), (dict(rope=None), L.LBW_ERR_INVALID),
+    (dict(pos=None), L.LBW_ERR_INVALID), (dict(bits=16), L.LBW_ERR_INVALID), (dict(dtype=3), L.LBW_ERR_INVALID),
+    (dict(dim=100), L.LBW_ERR_SHAPE), (dict(dim=264), L.LBW_ERR_SHAPE), (dict(dim=56), L.LBW_ERR_SHAPE),
+    (dict(heads=0), L.LBW_ERR_SHAPE), (dict(tokens=-1), L.LBW_ERR_SHAPE), (dict(x_tok=1001), L.LBW_ERR_ALIGN),
+    (dict(x=ctypes.c_void_p(4104)), L.LBW_ERR_ALIGN), (dict(rope=_rope(30)), L.LBW_ERR_SHAPE),
+    (dict(rope=_rope(32, 0)), L.LBW_ERR_SHAPE), (dict(rope=_rope(32, 1, 2)), L.LBW_ERR_INVALID),
+    (dict(rope=_rope(32, 1, 0, 1)), L.LBW_ERR_INVALID), (dict(rope=_rope(132)), L.LBW_ERR_SHAPE),
+    (dict(tokens=0, x=None, out=None, pos=None), L.LBW_OK)])
+def test_axial_rope_entry_checks(lib, change, status):
+    a = dict(x=P, x_tok=1024, x_head=64, out=P, out_tok=1024, out_head=64, tokens=5, heads=2, dim=64, dtype=0, pos=P,
+             bits=32, pos_tok=1, pos_axis=1, rope=_rope(), inverse=0)
+    a.update(change)
+    rc = lib.lbw_axial_rope(*a.values(), None)
+    assert rc == status
+    if status:
+        assert "axial_rope" in L.last_error()
+
+
+def _rows(**kw):
+    r = dict(x=4096, out=4096, gamma=0, x_tok=1024, x_head=64, out_row=1024, out_head=64, heads=2, gamma_f32=0)
+    r.update(kw)
+    return ctypes.byref(L.HeadRows(*r.values()))
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(q=None), L.LBW_ERR_INVALID), (dict(k=None), L.LBW_ERR_INVALID), (dict(q=_rows(x=0)), L.LBW_ERR_INVALID),
+    (dict(k=_rows(out=4098)), L.LBW_ERR_ALIGN), (dict(k=_rows(out_row=1020)), L.LBW_ERR_ALIGN),
+    (dict(v=_rows(heads=0)), L.LBW_ERR_SHAPE), (dict(q=_rows(gamma=4097)), L.LBW_ERR_ALIGN),
+    (dict(eps=-1.0), L.LBW_ERR_INVALID), (dict(eps=math.nan), L.LBW_ERR_INVALID), (dict(rows_bits=8), L.LBW_ERR_INVALID),
+    (dict(out_rows=-1), L.LBW_ERR_SHAPE), (dict(dim=12), L.LBW_ERR_SHAPE), (dict(tokens=0, q=_rows(x=0)), L.LBW_OK)])
+def test_qk_headnorm_rope_entry_checks(lib, change, status):
+    a = dict(q=_rows(), k=_rows(), v=None, tokens=5, dim=64, dtype=0, eps=1e-6, pos=P, bits=32, pos_tok=1, pos_axis=1,
+             rope=_rope(), rows=P, rows_bits=64, out_rows=9)
+    a.update(change)
+    assert lib.lbw_qk_headnorm_rope(*a.values(), None) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(q=None), L.LBW_ERR_INVALID), (dict(v=None), L.LBW_ERR_INVALID), (dict(out=None), L.LBW_ERR_INVALID),
+    (dict(cu_q=None), L.LBW_ERR_INVALID), (dict(dim=96), L.LBW_ERR_SHAPE), (dict(hk=3), L.LBW_ERR_SHAPE),
+    (dict(hk=0), L.LBW_ERR_SHAPE), (dict(n=-1), L.LBW_ERR_SHAPE), (dict(tk=1 << 31), L.LBW_ERR_SHAPE),
+    (dict(dtype=2), L.LBW_ERR_INVALID), (dict(scale=0.0), L.LBW_ERR_INVALID), (dict(scale=math.nan), L.LBW_ERR_INVALID),
+    (dict(scale=math.inf), L.LBW_ERR_INVALID), (dict(out_tok=1028), L.LBW_ERR_ALIGN),
+    (dict(out=ctypes.c_void_p(4104)), L.LBW_ERR_ALIGN), (dict(cu_k=ctypes.c_void_p(4098)), L.LBW_ERR_ALIGN),
+    (dict(tq=0), L.LBW_OK), (dict(n=0), L.LBW_OK)])
+def test_packed_attention_entry_checks(lib, change, status):
+    a = dict(q=P, q_tok=1024, q_head=64, k=P, k_tok=1024, k_head=64, v=P, v_tok=1024, v_head=64, out=P, out_tok=1024,
+             out_head=64, cu_q=P, cu_k=P, k_lens=None, n=2, tq=100, tk=100, hq=8, hk=2, dim=64, dtype=0, causal=1,
+             scale=0.1, max_q=0, ws=P, ws_bytes=1 << 40)
+    a.update(change)
+    assert lib.lbw_packed_attention(*a.values(), None) == status
+
+
+def test_packed_attention_refuses_a_small_workspace(lib):
+    n = ctypes.c_longlong(-1)
+    assert lib.lbw_packed_attention_workspace(1, 100000, 8, 2, 128, 1, 1, ctypes.byref(n)) == L.LBW_OK
+    assert n.value > 0
+    rc = lib.lbw_packed_attention(P, 1024, 128, P, 1024, 128, P, 1024, 128, P, 1024, 128, P, P, None, 1, 1, 100000, 8, 2,
+                                  128, 0, 1, 0.1, 1, P, n.value - 1, None)
+    assert rc == L.LBW_ERR_INVALID and "workspace" in L.last_error()
+    assert lib.lbw_packed_attention_workspace(1, 100, 8, 3, 128, 1, 1, ctypes.byref(n)) == L.LBW_ERR_SHAPE
+    assert lib.lbw_packed_attention_workspace(1, 100, 8, 2, 128, 1, 1, None) == L.LBW_ERR_INVALID
