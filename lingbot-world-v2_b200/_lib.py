@@ -8,6 +8,7 @@ shapes, RuntimeError for device/runtime failures.
 import ctypes
 import os
 import re
+import struct
 
 import torch
 
@@ -68,7 +69,7 @@ SIGNATURES = {
     "lbw_mx_linear_act": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp], _i),
     "lbw_axial_rope": ([_vp, _ll, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _vp, _i, _ll, _ll, _vp, _i, _vp], _i),
     "lbw_qk_headnorm_rope": ([_vp, _vp, _vp, _ll, _i, _i, _f, _vp, _i, _ll, _ll, _vp, _vp, _i, _ll, _vp], _i),
-    "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, ctypes.POINTER(_ll)], _i),
+    "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, ctypes.POINTER(_ll), ctypes.POINTER(_i)], _i),
     "lbw_packed_attention": ([_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _ll, _ll,
                               _i, _i, _i, _i, _i, _f, _i, _vp, _ll, _vp], _i),
     "lbw_vae_conv": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
@@ -145,10 +146,8 @@ def check(rc, what, launches=1):
     raise LbwError(msg)
 
 
-class HeadRows(ctypes.Structure):
-    """lbw_head_rows (include/lbw.h)."""
-    _fields_ = [("x", _vp), ("out", _vp), ("gamma", _vp), ("x_tok", _ll), ("x_head", _ll), ("out_row", _ll),
-                ("out_head", _ll), ("heads", _i), ("gamma_f32", _i)]
+# lbw_head_rows (include/lbw.h) as bytes: x, out, gamma, x_tok, x_head, out_row, out_head, heads, gamma_f32.
+HEAD_ROWS = struct.Struct("@PPPqqqqii")
 
 
 def ptr(t):
@@ -159,6 +158,11 @@ def ptr(t):
 
 def stream_of(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def raw_stream(device_index):
+    """stream_of as a plain integer: a tenth of its time, which counts in calls of a few microseconds."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def check_device_status(stream=None):

@@ -17,8 +17,11 @@
 // The pipeline (P written over S in TMEM and released in two halves, a running maximum that moves only when it grows by
 // more than 2^8, a quarter of the exponentials on the FMA pipe) is the chunk attention's, see attn.cu for its figures.
 // Rows that see no key (causal with fewer keys than queries, no keys at all) get zeros.
+#include <limits.h>
+
 #include "host_common.cuh"
 #include "packed_common.cuh"
+#include "packed_host.cuh"
 
 namespace lbw {
 
@@ -33,7 +36,7 @@ struct TileArgs {
   int pack;        // query heads side by side in a tile
   int tile_toks;   // tokens of a tile: 128 / pack
   int head_tiles;  // hq / pack
-  int short_rows;  // sequences with at most this many rows per kv head (nq * group) are another kernel's
+  int short_rows;  // sequences with at most this many rows per kv head (nq * group) are packed_split_kernel's
   int n_split;     // key ranges per window (> 1: partial results, merged by packed_merge_kernel)
   float* part_o;   // [n_split][tq * hq][D]
   float* part_ml;  // [n_split][tq * hq][2]
@@ -75,7 +78,9 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
       p_ready[2][2], o_done[2], done_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int found[2];
+  __shared__ int found;
+  __shared__ PackedSeq found_seq;
+  __shared__ int found_item;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
@@ -87,8 +92,9 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
       return (s.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
     }, b, l);
     if (lane == 0) {
-      found[0] = ok ? b : -1;
-      found[1] = (int)l;
+      found = ok;
+      found_item = (int)l;
+      if (ok) found_seq = packed_seq(a, b);
     }
   }
   if (threadIdx.x == 0) {
@@ -110,7 +116,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     fence_mbar_init();
   }
   __syncthreads();
-  if (found[0] < 0) return;  // the grid is an upper bound made from the row counts alone
+  if (!found) return;  // the grid is an upper bound made from the row counts alone
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -119,9 +125,9 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
   const Abort ab{status, &abort_flag};
 
   // The window: pairs of tiles of a sequence are taken from its end, where causal rows see most keys.
-  const PackedSeq sq = packed_seq(a, found[0]);
+  const PackedSeq sq = found_seq;
   const int n_pairs = (sq.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
-  const int tok0 = (n_pairs - 1 - found[1]) * 2 * ta.tile_toks;
+  const int tok0 = (n_pairs - 1 - found_item) * 2 * ta.tile_toks;
   const bool two = tok0 + ta.tile_toks < sq.nq;
   const int head0 = (int)(blockIdx.x % ta.head_tiles) * ta.pack;
   const int kv_head = head0 / a.group;
@@ -527,21 +533,33 @@ static int pick_pack(int group, long long avg) {
   return best;
 }
 
-// The call's launch plan, from the host's numbers alone.
+// Rows per kv head (queries x group) up to which a sequence is packed_split_kernel's, which has 16 in a unit.
+constexpr int SHORT_ROWS = 16;
+
+// The call's launch plan, from the host's numbers alone. The sequences' own lengths are on the device: where they may be
+// of both kinds, both kernels are launched and each takes its own.
 struct PackedPlan {
+  bool tiles, split;
+  long long split_rows;   // packed_split_kernel's limit
   TileArgs tile;
-  long long windows;   // upper bound of the tile kernel's windows
-  long long ws_floats; // workspace, fp32 values
+  long long windows;      // upper bound of the tile kernel's windows
+  long long tile_floats, split_floats;  // workspace, fp32 values
 };
 
-static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, int n_seqs) {
+static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, int n_seqs, int max_q) {
   PackedPlan p{};
   const int group = hq / hk;
+  const long long most = max_q > 0 && max_q < tq ? max_q : tq;
+  p.tiles = most * group > SHORT_ROWS;
+  p.split = !p.tiles || n_seqs > 1;
+  p.split_rows = p.tiles ? SHORT_ROWS : LLONG_MAX;  // (a sequence longer than max_q promised is still computed)
+  if (p.split) p.split_floats = split_workspace_floats(d);
+  if (!p.tiles) return p;
   const long long avg = n_seqs > 0 ? (tq + n_seqs - 1) / n_seqs : tq;
   p.tile.pack = pick_pack(group, avg > 0 ? avg : 1);
   p.tile.tile_toks = 128 / p.tile.pack;
   p.tile.head_tiles = hq / p.tile.pack;
-  p.tile.short_rows = 0;
+  p.tile.short_rows = p.split ? SHORT_ROWS : 0;
   long long pairs = tq / (2 * p.tile.tile_toks) + n_seqs;
   if (pairs > tq) pairs = tq;
   p.windows = pairs * p.tile.head_tiles;
@@ -550,7 +568,7 @@ static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, i
   if (split > key_tiles / 4) split = key_tiles / 4;
   if (split > 16) split = 16;
   p.tile.n_split = split < 1 ? 1 : (int)split;
-  if (p.tile.n_split > 1) p.ws_floats = (long long)p.tile.n_split * tq * hq * (d + 2);
+  if (p.tile.n_split > 1) p.tile_floats = (long long)p.tile.n_split * tq * hq * (d + 2);
   return p;
 }
 
@@ -568,12 +586,14 @@ static int check_packed(long long tq, long long tk, int hq, int hk, int d, int n
 extern "C" {
 
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
-                                   long long* bytes) {
+                                   long long* bytes, int* launches) {
   if (!bytes) return set_error(LBW_ERR_INVALID, "packed_attention_workspace: null pointer");
   const int err = check_packed(tq, tk, hq, hk, head_dim, n_seqs);
   if (err) return err;
-  (void)max_q;
-  *bytes = make_plan(tq, tk, hq, hk, head_dim, n_seqs).ws_floats * 4;
+  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q);
+  const bool any = tq > 0 && n_seqs > 0;
+  *bytes = any ? (p.tile_floats + p.split_floats) * 4 : 0;
+  if (launches) *launches = any ? (p.tiles ? 1 + (p.tile.n_split > 1) : 0) + (p.split ? 2 : 0) : 0;
   return LBW_OK;
 }
 
@@ -583,7 +603,6 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
                          int n_seqs, long long tq, long long tk, int hq, int hk, int head_dim, int dtype, int causal,
                          float softmax_scale, int max_q, void* workspace, long long ws_bytes, void* stream) {
   const char* who = "packed_attention";
-  (void)max_q;
   int err = check_packed(tq, tk, hq, hk, head_dim, n_seqs);
   if (err) return err;
   if (dtype != LBW_BF16 && dtype != LBW_FP16) return set_error(LBW_ERR_INVALID, "%s: dtype %d (bf16 or fp16)", who, dtype);
@@ -593,34 +612,45 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   if (!q || !out || !cu_q || !cu_k || (tk > 0 && (!k || !v))) return set_error(LBW_ERR_INVALID, "%s: null pointer", who);
   if (!aligned(cu_q, 4) || !aligned(cu_k, 4) || !aligned(k_lens, 4) || !aligned(out, 16) || out_tok % 8 || out_head % 8)
     return set_error(LBW_ERR_ALIGN, "%s: the output needs a 16-byte aligned pointer and strides", who);
-  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs);
+  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q);
   if (p.windows >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
-  if (p.ws_floats > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < p.ws_floats * 4))
-    return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who,
-                     p.ws_floats * 4, ws_bytes);
+  const long long need = (p.tile_floats + p.split_floats) * 4;
+  if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
+    return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who, need,
+                     ws_bytes);
   int* st = device_status(&err);
   if (!st) return err;
-  const CUtensorMapDataType ty = dtype == LBW_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap tmQ, tmK, tmV;
-  if ((err = make_tmap_3d(&tmQ, q, ty, head_dim, hq, tq, q_head, q_tok, p.tile.pack, p.tile.tile_toks))) return err;
-  if (tk > 0) {
-    if ((err = make_tmap_3d(&tmK, k, ty, head_dim, hk, tk, k_head, k_tok, 1, pa::BN))) return err;
-    if ((err = make_tmap_3d(&tmV, v, ty, head_dim, hk, tk, v_head, v_tok, 1, pa::BN))) return err;
-  } else {
-    tmK = tmV = tmQ;  // no key tile is ever loaded
-  }
-  PackedArgs a{cu_q, cu_k, k_lens, n_seqs, (int)tq, (int)tk, hq, hk, hq / hk, causal != 0,
-               softmax_scale * 1.4426950408889634f, out, out_tok, out_head};
-  TileArgs ta = p.tile;
-  ta.part_o = reinterpret_cast<float*>(workspace);
-  ta.part_ml = ta.part_o ? ta.part_o + (long long)ta.n_split * tq * hq * head_dim : nullptr;
-  const dim3 grid((unsigned)p.windows, ta.n_split);
+  const PackedArgs a{cu_q, cu_k, k_lens, n_seqs, (int)tq, (int)tk, hq, hk, hq / hk, causal != 0,
+                     softmax_scale * 1.4426950408889634f, out, out_tok, out_head};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128)
-    return dtype == LBW_FP16 ? launch_tiles<128, true>(tmQ, tmK, tmV, a, ta, grid, st, s)
-                             : launch_tiles<128, false>(tmQ, tmK, tmV, a, ta, grid, st, s);
-  return dtype == LBW_FP16 ? launch_tiles<64, true>(tmQ, tmK, tmV, a, ta, grid, st, s)
-                           : launch_tiles<64, false>(tmQ, tmK, tmV, a, ta, grid, st, s);
+  float* ws = reinterpret_cast<float*>(workspace);
+  if (p.tiles) {
+    const CUtensorMapDataType ty = dtype == LBW_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap tmQ, tmK, tmV;
+    if ((err = make_tmap_3d(&tmQ, q, ty, head_dim, hq, tq, q_head, q_tok, p.tile.pack, p.tile.tile_toks))) return err;
+    if (tk > 0) {
+      if ((err = make_tmap_3d(&tmK, k, ty, head_dim, hk, tk, k_head, k_tok, 1, pa::BN))) return err;
+      if ((err = make_tmap_3d(&tmV, v, ty, head_dim, hk, tk, v_head, v_tok, 1, pa::BN))) return err;
+    } else {
+      tmK = tmV = tmQ;  // no key tile is ever loaded
+    }
+    TileArgs ta = p.tile;
+    ta.part_o = ws;
+    ta.part_ml = ws ? ws + (long long)ta.n_split * tq * hq * head_dim : nullptr;
+    const dim3 grid((unsigned)p.windows, ta.n_split);
+    if (head_dim == 128)
+      err = dtype == LBW_FP16 ? launch_tiles<128, true>(tmQ, tmK, tmV, a, ta, grid, st, s)
+                              : launch_tiles<128, false>(tmQ, tmK, tmV, a, ta, grid, st, s);
+    else
+      err = dtype == LBW_FP16 ? launch_tiles<64, true>(tmQ, tmK, tmV, a, ta, grid, st, s)
+                              : launch_tiles<64, false>(tmQ, tmK, tmV, a, ta, grid, st, s);
+    if (err) return err;
+  }
+  if (!p.split) return LBW_OK;
+  if (!aligned(q, 16) || q_tok % 8 || q_head % 8)
+    return set_error(LBW_ERR_ALIGN, "%s: q needs a 16-byte aligned pointer and strides", who);
+  return launch_split(k, k_tok, k_head, v, v_tok, v_head, a, head_dim, dtype, q, q_tok, q_head, p.split_rows,
+                      ws + p.tile_floats, st, s);
 }
 
 }  // extern "C"

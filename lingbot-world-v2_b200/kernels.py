@@ -6,12 +6,13 @@ allocated here.
 """
 import contextlib
 import ctypes
+import functools
 import math
 
 import torch
 
 from . import _lib
-from ._lib import HeadRows, check, load, ptr, require_cuda, stream_of
+from ._lib import HEAD_ROWS, check, load, ptr, raw_stream, require_cuda, stream_of
 
 BF16 = torch.bfloat16
 HEAD_DIM = 128
@@ -742,56 +743,61 @@ def transpose_bf16(x, ldx, rows, cols, out, ldo):
 DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # lbw_dtype (include/lbw.h)
 
 
-def _same_device(who, *tensors):
-    """The device of all the given tensors (None skipped); these operators have no gradient."""
-    require_cuda(*tensors)
-    given = [t for t in tensors if t is not None]
-    if any(t.device != given[0].device for t in given):
-        raise ValueError(f"{who}: tensors on different devices")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
-        raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or with detached tensors")
-    return given[0].device
+def _device_index(who, *tensors):
+    """Index of the CUDA device that holds all the given tensors (None skipped); these operators have no gradient."""
+    dev = tensors[0].get_device()
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None:
+            if dev < 0 or t.get_device() < 0:
+                require_cuda(*tensors)
+            if t.get_device() != dev:
+                raise ValueError(f"{who}: tensors on different devices")
+            if grad and t.requires_grad:
+                raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or with detached tensors")
+    return dev
 
 
-def _on(device):
-    """Context in which `device` is the current one (the library launches on the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _on(dev):
+    """Context in which device `dev` is the current one (the library launches on the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev else torch.cuda.device(dev)
 
 
-def _heads3(who, name, t, dtype=None, dim=None):
-    """[tokens, heads, head_dim] view of a [tokens, heads, head_dim] or [1, tokens, heads, head_dim] tensor."""
-    if t.dim() == 4 and t.shape[0] == 1:
-        t = t[0]
-    if t.dim() != 3 or t.shape[1] < 1:
+def _rows3(who, name, t, dtype=None, dim=None, written=False):
+    """(tokens, heads, head_dim, token stride, head stride) of a [tokens, heads, head_dim] or [1, tokens, heads,
+    head_dim] tensor with a contiguous head_dim."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 4 and shape[0] == 1:
+        shape, stride = shape[1:], stride[1:]
+    if len(shape) != 3 or shape[1] < 1:
         raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if t.dtype != dtype and dtype is not None:
+    if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
-    if dim is not None and t.shape[2] != dim:
-        raise ValueError(f"{who}: head_dim of {name} is {t.shape[2]}, expected {dim}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if dim is not None and shape[2] != dim:
+        raise ValueError(f"{who}: head_dim of {name} is {shape[2]}, expected {dim}")
+    if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"{who}: {name} needs a contiguous head_dim")
-    return t
-
-
-def _writable(who, name, t):
-    """Refuses an output of which two elements share memory through a stride of zero."""
-    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+    if written and ((stride[0] == 0 and shape[0] > 1) or (stride[1] == 0 and shape[1] > 1)):
         raise ValueError(f"{who}: {name} is an expanded tensor")
-    return t
+    return (*shape, stride[0], stride[1])
 
 
 def _positions(who, positions, tokens, rope):
-    if positions.dim() == 1:
-        positions = positions[:, None]
-    if positions.dim() != 2 or positions.shape[0] != tokens or positions.shape[1] != rope.axes:
+    """(pointer, bits, token stride, axis stride) of [tokens, axes] (or [tokens]) positions."""
+    shape, stride = positions.shape, positions.stride()
+    if len(shape) == 1:
+        shape, stride = (shape[0], 1), (stride[0], 1)
+    if len(shape) != 2 or shape[0] != tokens or shape[1] != rope.axes:
         raise ValueError(f"{who}: positions must be [{tokens}, {rope.axes}], got {tuple(positions.shape)}")
-    return positions, _index_bits(who, "positions", positions)
+    return positions.data_ptr(), _index_bits(who, "positions", positions), stride[0], stride[1]
 
 
 def _index_bits(who, name, t):
-    if t.dtype not in (torch.int32, torch.int64):
+    if t.dtype == torch.int64:
+        return 64
+    if t.dtype != torch.int32:
         raise ValueError(f"{who}: {name} must be int32 or int64, got {t.dtype}")
-    return 32 if t.dtype == torch.int32 else 64
+    return 32
 
 
 def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
@@ -802,32 +808,35 @@ def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
     who = "axial_rope"
     if _tracing(_eager):
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            out = torch.empty_like(x)
         _op(who)(x, positions, list(rope.sections), rope.theta, rope.layout, rope.spectrum, list(rope.scale),
                  bool(inverse), out)
         return out
-    dev = _same_device(who, x, positions, out)
-    if x.dtype not in DTYPES:
-        raise ValueError(f"{who}: x is {x.dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
-    x3 = _heads3(who, "x", x)
-    tokens, heads, dim = x3.shape
+    dev = _device_index(who, x, positions, out)
+    dtype = x.dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"{who}: x is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
+    tokens, heads, dim, x_tok, x_head = _rows3(who, "x", x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    o3 = _writable(who, "out", _heads3(who, "out", out, x.dtype, dim))
-    if o3.shape != x3.shape:
+        out = torch.empty_like(x)
+    o_tokens, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
+    if o_tokens != tokens or o_heads != heads:
         raise ValueError(f"{who}: out is {tuple(out.shape)}, x {tuple(x.shape)}")
-    pos, bits = _positions(who, positions, tokens, rope)
+    pos = _positions(who, positions, tokens, rope)
     with _on(dev):
-        check(load().lbw_axial_rope(x3.data_ptr(), x3.stride(0), x3.stride(1), o3.data_ptr(), o3.stride(0),
-                                    o3.stride(1), tokens, heads, dim, DTYPES[x.dtype], pos.data_ptr(), bits,
-                                    pos.stride(0), pos.stride(1), rope.ref, int(bool(inverse)), stream_of(dev)),
-              who, launches=1 if tokens else 0)
+        check(load().lbw_axial_rope(x.data_ptr(), x_tok, x_head, out.data_ptr(), o_tok, o_head, tokens, heads, dim,
+                                    DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0, raw_stream(dev)), who,
+              launches=1 if tokens else 0)
     return out
 
 
-def _head_rows(x, out, gamma):
-    return HeadRows(x.data_ptr(), out.data_ptr(), 0 if gamma is None else gamma.data_ptr(), x.stride(0), x.stride(1),
-                    out.stride(0), out.stride(1), x.shape[1], int(gamma is not None and gamma.dtype == torch.float32))
+def _gain(who, name, g, dtype, dim):
+    """(pointer, is fp32) of a gain [dim]."""
+    if g is None:
+        return 0, 0
+    if g.shape != (dim,) or (g.dtype != dtype and g.dtype != torch.float32) or not g.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous [{dim}] {dtype} or fp32, got {tuple(g.shape)} {g.dtype}")
+    return g.data_ptr(), 1 if g.dtype == torch.float32 else 0
 
 
 def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_out=None, k_out=None, v=None,
@@ -840,69 +849,73 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
     write none. q_out may be q and, without k_rows, k_out may be k."""
     who = "qk_headnorm_rope"
     if _tracing(_eager):
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+        q_out = torch.empty_like(q) if q_out is None else q_out
+        k_out = torch.empty_like(k) if k_out is None else k_out
         r = rope
         _op(who)(q, k, gamma_q, gamma_k, float(eps), positions, list(r.sections) if r else [], r.theta if r else 1.0,
                  r.layout if r else "", r.spectrum if r else "", list(r.scale) if r else [], q_out, k_out, v, v_out,
                  k_rows)
         return q_out, k_out
-    dev = _same_device(who, q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows)
-    if q.dtype not in DTYPES:
-        raise ValueError(f"{who}: q is {q.dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
-    q3 = _heads3(who, "q", q)
-    tokens, _, dim = q3.shape
-    k3 = _heads3(who, "k", k, q.dtype, dim)
-    if k3.shape[0] != tokens:
-        raise ValueError(f"{who}: {tokens} rows of q, {k3.shape[0]} of k")
-    for name, g in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
-        if g is not None and (g.shape != (dim,) or g.dtype not in (q.dtype, torch.float32) or not g.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be contiguous [{dim}] {q.dtype} or fp32, got {tuple(g.shape)} {g.dtype}")
+    dev = _device_index(who, q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows)
+    dtype = q.dtype
+    if dtype not in DTYPES:
+        raise ValueError(f"{who}: q is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
     if (positions is None) != (rope is None):
         raise ValueError(f"{who}: give positions and rope, or neither")
     if (v is None) != (v_out is None) or (v is not None and k_rows is None):
         raise ValueError(f"{who}: v is copied to the rows k_rows of v_out: give all three, or no v")
     if k_rows is not None and k_out is None:
         raise ValueError(f"{who}: k_rows name rows of k_out: give it")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=dev) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=dev) if k_out is None else k_out
-    qo = _writable(who, "q_out", _heads3(who, "q_out", q_out, q.dtype, dim))
-    ko = _writable(who, "k_out", _heads3(who, "k_out", k_out, q.dtype, dim))
-    if qo.shape != q3.shape or ko.shape[1] != k3.shape[1] or (k_rows is None and ko.shape[0] != tokens):
+    tokens, hq, dim, q_tok, q_head = _rows3(who, "q", q)
+    k_tokens, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
+    if k_tokens != tokens:
+        raise ValueError(f"{who}: {tokens} rows of q, {k_tokens} of k")
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    k_out = torch.empty_like(k) if k_out is None else k_out
+    qo_rows, qo_heads, _, qo_row, qo_head = _rows3(who, "q_out", q_out, dtype, dim, written=True)
+    ko_rows, ko_heads, _, ko_row, ko_head = _rows3(who, "k_out", k_out, dtype, dim, written=True)
+    if qo_rows != tokens or qo_heads != hq or ko_heads != hk or (k_rows is None and ko_rows != tokens):
         raise ValueError(f"{who}: q_out {tuple(q_out.shape)} / k_out {tuple(k_out.shape)} do not match q, k")
-    rows_bits, seg_v = 0, None
+    gq, gq_f32 = _gain(who, "gamma_q", gamma_q, dtype, dim)
+    gk, gk_f32 = _gain(who, "gamma_k", gamma_k, dtype, dim)
+    seg_q = HEAD_ROWS.pack(q.data_ptr(), q_out.data_ptr(), gq, q_tok, q_head, qo_row, qo_head, hq, gq_f32)
+    seg_k = HEAD_ROWS.pack(k.data_ptr(), k_out.data_ptr(), gk, k_tok, k_head, ko_row, ko_head, hk, gk_f32)
+    seg_v, rows, rows_bits = None, None, 0
     if k_rows is not None:
-        rows_bits = _index_bits(who, "k_rows", k_rows)
+        rows, rows_bits = k_rows.data_ptr(), _index_bits(who, "k_rows", k_rows)
         if k_rows.shape != (tokens,) or not k_rows.is_contiguous():
             raise ValueError(f"{who}: k_rows must be contiguous [{tokens}], got {tuple(k_rows.shape)}")
     if v is not None:
-        v3 = _heads3(who, "v", v, q.dtype, dim)
-        vo = _writable(who, "v_out", _heads3(who, "v_out", v_out, q.dtype, dim))
-        if v3.shape[0] != tokens or vo.shape[1] != v3.shape[1] or vo.shape[0] != ko.shape[0]:
+        v_tokens, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
+        vo_rows, vo_heads, _, vo_row, vo_head = _rows3(who, "v_out", v_out, dtype, dim, written=True)
+        if v_tokens != tokens or vo_heads != hv or vo_rows != ko_rows:
             raise ValueError(f"{who}: v {tuple(v.shape)} / v_out {tuple(v_out.shape)} do not match q and k_out")
-        seg_v = ctypes.byref(_head_rows(v3, vo, None))
-    pos, pos_bits, st0, st1 = None, 32, 0, 0
-    if rope is not None:
-        p2, pos_bits = _positions(who, positions, tokens, rope)
-        pos, st0, st1 = p2.data_ptr(), p2.stride(0), p2.stride(1)
+        seg_v = HEAD_ROWS.pack(v.data_ptr(), v_out.data_ptr(), 0, v_tok, v_head, vo_row, vo_head, hv, 0)
+    pos = (None, 32, 0, 0) if rope is None else _positions(who, positions, tokens, rope)
     with _on(dev):
-        check(load().lbw_qk_headnorm_rope(ctypes.byref(_head_rows(q3, qo, gamma_q)),
-                                          ctypes.byref(_head_rows(k3, ko, gamma_k)), seg_v, tokens, dim,
-                                          DTYPES[q.dtype], float(eps), pos, pos_bits, st0, st1,
-                                          rope.ref if rope is not None else None, ptr(k_rows), rows_bits, ko.shape[0],
-                                          stream_of(dev)), who, launches=1 if tokens else 0)
+        check(load().lbw_qk_headnorm_rope(seg_q, seg_k, seg_v, tokens, dim, DTYPES[dtype], eps, *pos,
+                                          None if rope is None else rope.ref, rows, rows_bits, ko_rows,
+                                          raw_stream(dev)), who, launches=1 if tokens else 0)
     return q_out, k_out
+
+
+@functools.lru_cache(4096)
+def _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, dev):
+    """(workspace bytes, kernels launched) of a call with these sizes on device dev."""
+    b, k = ctypes.c_longlong(0), ctypes.c_int(0)
+    with torch.cuda.device(dev):
+        check(load().lbw_packed_attention_workspace(tq, tk, hq, hk, dim, n, max_q, ctypes.byref(b), ctypes.byref(k)),
+              "packed_attention_workspace")
+    return b.value, k.value
 
 
 def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=None):
     """Workspace (uint8) of packed_attention calls with these sizes, or None when they need none. Calls that may overlap
     (other streams, graphs replayed side by side) need one each; packed_attention makes its own when given none."""
-    n = ctypes.c_longlong(0)
     device = torch.device(device)
-    with torch.cuda.device(device):
-        check(load().lbw_packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0),
-                                                    ctypes.byref(n)), "packed_attention_workspace")
-    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+    dev = torch.cuda.current_device() if device.index is None else device.index
+    n, _ = _packed_attention_plan(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0), dev)
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scale=None, out=None, max_q=None,
@@ -917,38 +930,44 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
     who = "packed_attention"
     if _tracing(_eager):
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = torch.empty_like(q)
         scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
         _op(who)(q, k, v, cu_q, cu_k, k_lens, bool(causal), float(scale), out, int(max_q or 0))
         return out
-    dev = _same_device(who, q, k, v, cu_q, cu_k, k_lens, out, workspace)
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"{who}: q is {q.dtype}, expected bf16 or fp16")
-    q3 = _heads3(who, "q", q)
-    tq, hq, dim = q3.shape
-    k3, v3 = _heads3(who, "k", k, q.dtype, dim), _heads3(who, "v", v, q.dtype, dim)
-    tk, hk = k3.shape[0], k3.shape[1]
-    if v3.shape != k3.shape:
+    dev = _device_index(who, q, k, v, cu_q, cu_k, k_lens, out, workspace)
+    dtype = q.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"{who}: q is {dtype}, expected bf16 or fp16")
+    tq, hq, dim, q_tok, q_head = _rows3(who, "q", q)
+    tk, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
+    v_rows, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
+    if v_rows != tk or hv != hk:
         raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
     for name, t, want in (("cu_q", cu_q, n + 1), ("cu_k", cu_k, n + 1), ("k_lens", k_lens, n)):
         if t is not None and (n < 0 or t.dtype != torch.int32 or t.shape != (want,) or not t.is_contiguous()):
             raise ValueError(f"{who}: {name} must be contiguous int32 [{max(want, 0)}], got {tuple(t.shape)} {t.dtype}")
-    if max_q is not None and max_q < 0:
+    if max_q is None:
+        max_q = 0
+    elif max_q < 0:
         raise ValueError(f"{who}: max_q {max_q}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    o3 = _writable(who, "out", _heads3(who, "out", out, q.dtype, dim))
-    if o3.shape != q3.shape:
+        out = torch.empty_like(q)
+    o_rows, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
+    if o_rows != tq or o_heads != hq:
         raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
-    if workspace is None:
-        workspace = packed_attention_workspace(tq, tk, hq, hk, dim, n, dev, max_q)
+    ws_bytes, launches = _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, dev)
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError(f"{who}: the workspace must be contiguous")
+        ws_bytes = workspace.numel() * workspace.element_size()
+    elif ws_bytes:
+        workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
     with _on(dev):
         check(load().lbw_packed_attention(
-            q3.data_ptr(), q3.stride(0), q3.stride(1), k3.data_ptr(), k3.stride(0), k3.stride(1), v3.data_ptr(),
-            v3.stride(0), v3.stride(1), o3.data_ptr(), o3.stride(0), o3.stride(1), cu_q.data_ptr(), cu_k.data_ptr(),
-            ptr(k_lens), n, tq, tk, hq, hk, dim, DTYPES[q.dtype], int(bool(causal)), scale, int(max_q or 0),
-            ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(), stream_of(dev)),
-            who)
+            q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head, out.data_ptr(),
+            o_tok, o_head, cu_q.data_ptr(), cu_k.data_ptr(), None if k_lens is None else k_lens.data_ptr(), n, tq, tk,
+            hq, hk, dim, DTYPES[dtype], 1 if causal else 0, scale, max_q,
+            None if workspace is None else workspace.data_ptr(), ws_bytes, raw_stream(dev)), who, launches=launches)
     return out
