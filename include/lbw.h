@@ -284,10 +284,11 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
  * head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A non-finite value in a visible key or value reaches the
  * rows that see it; in a value row it also reaches rows of the same sequence that stand before it by less than 128 keys.
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
- * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (launches, if
- * not NULL, gets the number of kernels that such a call enqueues). */
+ * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
+ * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels
+ * that such a call enqueues). */
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
-                                   long long* bytes, int* launches);
+                                   int same_lens, long long* bytes, int* launches);
 int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const void* k, long long k_tok,
                          long long k_head, const void* v, long long v_tok, long long v_head, void* out,
                          long long out_tok, long long out_head, const int* cu_q, const int* cu_k, const int* k_lens,

@@ -69,7 +69,7 @@ SIGNATURES = {
     "lbw_mx_linear_act": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp], _i),
     "lbw_axial_rope": ([_vp, _ll, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _vp, _i, _ll, _ll, _vp, _i, _vp], _i),
     "lbw_qk_headnorm_rope": ([_vp, _vp, _vp, _ll, _i, _i, _f, _vp, _i, _ll, _ll, _vp, _vp, _i, _ll, _vp], _i),
-    "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, ctypes.POINTER(_ll), ctypes.POINTER(_i)], _i),
+    "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, _i, ctypes.POINTER(_ll), ctypes.POINTER(_i)], _i),
     "lbw_packed_attention": ([_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _ll, _ll,
                               _i, _i, _i, _i, _i, _f, _i, _vp, _ll, _vp], _i),
     "lbw_vae_conv": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),

@@ -11,9 +11,11 @@
 //
 // Bound: bytes (each value read once and written once, ~7 flops each). A head is D / 8 "units" of 8 values, one per
 // lane: unit u holds the pairs 4u .. 4u + 3, which are 8 neighbouring values (interleaved pairs: one 16-byte access)
-// or two runs of 4 values R apart (half layout: two 8-byte accesses), so a pair never crosses lanes and the only
-// exchange is the norm's sum over the head's 8, 16 or 32 lanes. A lane has the same unit of every head that it visits:
-// it computes its four angles once for a token and uses them for all of its heads.
+// or two runs of 4 values R apart (half layout: two 8-byte accesses), so a pair never crosses lanes and the only exchange
+// is the norm's sum over the head's 8, 16 or 32 lanes. The lanes of a head stay with one token: each computes its four
+// angles once and uses them, with the gains multiplied in, for the same unit of all of the token's heads.
+// Measured (B200, 10,800 tokens, 128-wide heads, bf16): norm of 40 + 40 heads out of the fused projection 78 us (442 MB,
+// 5.7 TB/s, 87% of a plain copy's rate; 84 us in the half layout), rotation of 120 heads 109-114 us (5.8-6.1 TB/s).
 #include <cuda_fp16.h>
 
 #include "host_common.cuh"
@@ -23,7 +25,8 @@ namespace lbw {
 
 namespace hr {
 constexpr int THREADS = 128;
-constexpr int UN = 4;  // heads loaded ahead by a lane group
+constexpr int MINB = 6;  // blocks per SM: 80 registers; 8 blocks spill and are 5% slower, 4 have too few loads in flight
+constexpr int UN = 4;    // heads loaded ahead by a lane group; 2 or 8 are 5-10% slower
 }  // namespace hr
 
 // One group of heads of every token: q, k or v. Strides in elements.
@@ -34,15 +37,13 @@ struct HeadSeg {
   long long xs_tok, xs_head, os_tok, os_head;
   int heads;
   int gamma_f32;
-  int mode;     // 0: norm (if the kernel norms) + rotation, 1: plain copy
-  int scatter;  // 1: the token's output row is rows[token]
 };
 
 struct HeadArgs {
   HeadSeg seg[3];
   long long tokens;
-  int dim, units, group;  // units = dim / 8, group = lanes of a head (8, 16 or 32)
-  int chunk, chunks;      // heads per work item, items per token
+  int dim, units;     // units = dim / 8
+  int chunk, chunks;  // heads per work item, items per token
   float eps;
   const void* pos;
   int pos_bits;
@@ -135,114 +136,146 @@ LBW_DEV long long load_index(const void* p, int bits, long long i) {
   return bits == 64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
 
-// Heads [h0, h1) of one segment of one token, `slots` heads at a time per warp and UN of those loaded ahead (the loads
-// of all UN come before the first store: input and output may be the same tensor).
-template <typename T, bool NORM, bool HALF>
-LBW_DEV void head_run(const HeadArgs& a, const HeadSeg& g, long long tok, long long row, int h0, int h1, int sub, int u,
-                      int slots, int o0, int o1, bool rotated, const float (&c)[4], const float (&s)[4],
-                      const float (&gain)[8]) {
-  const T* xt = reinterpret_cast<const T*>(g.x) + tok * g.xs_tok;
-  T* ot = reinterpret_cast<T*>(g.out) + row * g.os_tok;
-  const bool on = u < a.units;
+// Gains of a unit (1 without any).
+template <typename T, bool HALF>
+LBW_DEV void load_gain(float (&gain)[8], const HeadSeg& g, bool on, int o0, int o1) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) gain[e] = 1.f;
+  if (!g.gamma || !on) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int d = e < 4 ? o0 + e : o1 + e - 4;
+    gain[e] = g.gamma_f32 ? reinterpret_cast<const float*>(g.gamma)[d]
+                          : load_as_float(reinterpret_cast<const T*>(g.gamma) + d);
+  }
+}
+
+// Heads [h0, h1) of one segment of the lane group's token, UN at a time: their loads all come before the first store
+// (input and output may be the same tensor). The factors of the unit's pairs, (a, b) -> (a w0 - b w1, a w2 + b w3),
+// hold the gains.
+template <typename T, bool NORM, bool HALF, int G>
+LBW_DEV void head_run(const HeadArgs& a, const HeadSeg& g, long long tok, long long row, bool on, int h0, int h1, int o0,
+                      int o1, bool rotated, const float (&c)[4], const float (&s)[4]) {
+  const T* px = reinterpret_cast<const T*>(g.x) + tok * g.xs_tok + h0 * g.xs_head;
+  T* po = reinterpret_cast<T*>(g.out) + row * g.os_tok + h0 * g.os_head;
+  float w[4][4];
+  {
+    float gain[8];
+    if constexpr (NORM) load_gain<T, HALF>(gain, g, on, o0, o1);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float g0 = NORM ? gain[HALF ? p : 2 * p] : 1.f, g1 = NORM ? gain[HALF ? p + 4 : 2 * p + 1] : 1.f;
+      w[p][0] = g0 * c[p];
+      w[p][1] = g1 * s[p];
+      w[p][2] = g0 * s[p];
+      w[p][3] = g1 * c[p];
+    }
+  }
   const float inv_d = 1.f / (float)a.dim;
-  for (int h = h0 + sub; h - sub < h1; h += slots * hr::UN) {
+  for (int h = h0; h < h1; h += hr::UN) {
     Vec8<T> r[hr::UN];
 #pragma unroll
     for (int i = 0; i < hr::UN; ++i) {
       r[i] = Vec8<T>{};
-      if (on && h + i * slots < h1) load8<T, HALF>(r[i], xt + (h + i * slots) * g.xs_head, o0, o1);
+      if (on && h + i < h1) load8<T, HALF>(r[i], px + i * g.xs_head, o0, o1);
     }
 #pragma unroll
     for (int i = 0; i < hr::UN; ++i) {
-      if (h - sub + i * slots >= h1) break;  // warp-uniform
-      if (g.mode == 0 && (NORM || rotated)) {  // (what is only copied keeps its bits, a NaN's too)
-        float f[8];
-        unpack8(r[i], f);
-        if constexpr (NORM) {
-          float ss = 0.f;
+      float f[8];
+      unpack8(r[i], f);
+      float k = 1.f;
+      if constexpr (NORM) {
+        float ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-          for (int o = a.group >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float k = rsqrtf(fmaf(ss, inv_d, a.eps));
+        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = f[e] * k * gain[e];
-        }
-        if (rotated) {
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const int lo = HALF ? p : 2 * p, hi = HALF ? p + 4 : 2 * p + 1;
-            const float x0 = f[lo], x1 = f[hi];
-            f[lo] = x0 * c[p] - x1 * s[p];
-            f[hi] = x0 * s[p] + x1 * c[p];
-          }
-        }
-        pack8(r[i], f);
+        for (int o = G / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        k = rsqrtf(fmaf(ss, inv_d, a.eps));
       }
-      if (on && h + i * slots < h1) store8<T, HALF>(r[i], ot + (h + i * slots) * g.os_head, o0, o1);
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int lo = HALF ? p : 2 * p, hi = HALF ? p + 4 : 2 * p + 1;
+        const float x0 = f[lo], x1 = f[hi];
+        f[lo] = x0 * w[p][0];
+        f[hi] = x1 * w[p][3];
+        if (rotated) {
+          f[lo] = fmaf(-x1, w[p][1], f[lo]);
+          f[hi] = fmaf(x0, w[p][2], f[hi]);
+        }
+        if constexpr (NORM) {
+          f[lo] *= k;
+          f[hi] *= k;
+        }
+      }
+      if (NORM || rotated) pack8(r[i], f);  // (what is only copied keeps its bits, a NaN's too)
+      if (on && h + i < h1) store8<T, HALF>(r[i], po + i * g.os_head, o0, o1);
     }
+    px += hr::UN * g.xs_head;
+    po += hr::UN * g.os_head;
   }
 }
 
-// Work item = (token, chunk of the token's q | k | v heads), one warp each, grid-stride.
-template <typename T, bool NORM, bool HALF>
-__global__ void __launch_bounds__(hr::THREADS) head_rope_kernel(const __grid_constant__ HeadArgs a) {
-  __shared__ unsigned long long step[128];
-  __shared__ unsigned char axis[128];
+template <typename T, bool HALF>
+LBW_DEV void head_copy(const HeadSeg& g, long long tok, long long row, bool on, int h0, int h1, int o0, int o1) {
+  const T* px = reinterpret_cast<const T*>(g.x) + tok * g.xs_tok;
+  T* po = reinterpret_cast<T*>(g.out) + row * g.os_tok;
+  if (!on) return;
+  for (int h = h0; h < h1; ++h) {
+    Vec8<T> r;
+    load8<T, HALF>(r, px + h * g.xs_head, o0, o1);
+    store8<T, HALF>(r, po + h * g.os_head, o0, o1);
+  }
+}
+
+// Work item = (32 / G neighbouring tokens, chunk of the q | k | v heads), one warp each, grid-stride; a group of G lanes
+// has one token.
+template <typename T, bool NORM, bool HALF, int G>
+__global__ void __launch_bounds__(hr::THREADS, hr::MINB) head_rope_kernel(const __grid_constant__ HeadArgs a) {
+  __shared__ __align__(16) unsigned long long step[128];
+  __shared__ __align__(4) unsigned char axis[128];
   for (int i = threadIdx.x; i < a.rope.pairs; i += hr::THREADS) {
     step[i] = a.rope.step[i];
     axis[i] = a.rope.axis[i];
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  const int slots = 32 / a.group;
-  const int u = lane & (a.group - 1), sub = lane / a.group;
+  const int u = lane & (G - 1), sub = lane / G;
   const bool rotated = 4 * u < a.rope.pairs;
   const int o0 = HALF && rotated ? 4 * u : 8 * u;
   const int o1 = HALF && rotated ? a.rope.pairs + 4 * u : 8 * u + 4;
-  float gain[2][8];
-  if constexpr (NORM) {
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = e < 4 ? o0 + e : o1 + e - 4;
-        gain[w][e] = 1.f;
-        if (a.seg[w].gamma && u < a.units)
-          gain[w][e] = a.seg[w].gamma_f32 ? reinterpret_cast<const float*>(a.seg[w].gamma)[d]
-                                          : load_as_float(reinterpret_cast<const T*>(a.seg[w].gamma) + d);
-      }
-  }
   const int hq = a.seg[0].heads, hk = a.seg[1].heads, hv = a.seg[2].heads;
-  const long long items = a.tokens * a.chunks;
+  const long long items = (a.tokens + 32 / G - 1) / (32 / G) * a.chunks;
   const long long stride = (long long)gridDim.x * (hr::THREADS / 32);
   for (long long it = (long long)blockIdx.x * (hr::THREADS / 32) + (threadIdx.x >> 5); it < items; it += stride) {
-    const long long tok = it / a.chunks;
-    const int lo = (int)(it - tok * a.chunks) * a.chunk;
+    const long long block = it / a.chunks;
+    const long long tok = block * (32 / G) + sub;
+    const bool here = tok < a.tokens;
+    const bool on = here && u < a.units;
+    const int lo = (int)(it - block * a.chunks) * a.chunk;
     const int hi = min(lo + a.chunk, hq + hk + hv);
     float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (rotated && lo < hq + hk) {
+    if (rotated && here && lo < hq + hk) {
+      const uchar4 ax = *reinterpret_cast<const uchar4*>(axis + 4 * u);
+      const unsigned char axs[4] = {ax.x, ax.y, ax.z, ax.w};
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        const int i = 4 * u + p;
-        const long long ps = load_index(a.pos, a.pos_bits, tok * a.ps_tok + axis[i] * a.ps_axis);
-        const unsigned long long turns = (unsigned long long)ps * step[i];
+        const long long ps = load_index(a.pos, a.pos_bits, tok * a.ps_tok + axs[p] * a.ps_axis);
+        const unsigned long long turns = (unsigned long long)ps * step[4 * u + p];
         sincospif((float)(int)(turns >> 32) * 4.656612873077393e-10f, &s[p], &c[p]);  // 2^-31: half turns in [-1, 1]
       }
     }
+    if (lo < hq) head_run<T, NORM, HALF, G>(a, a.seg[0], tok, tok, on, lo, min(hi, hq), o0, o1, rotated, c, s);
+    if (hi <= hq) continue;
     long long row = tok;
-    bool keep = true;
-    if (a.rows) {
+    bool keep = on;
+    if (a.rows && here) {
       row = load_index(a.rows, a.rows_bits, tok);
-      keep = row >= 0 && row < a.out_rows;
+      keep = on && row >= 0 && row < a.out_rows;
     }
-    if (lo < hq)
-      head_run<T, NORM, HALF>(a, a.seg[0], tok, tok, lo, min(hi, hq), sub, u, slots, o0, o1, rotated, c, s, gain[0]);
-    if (hi > hq && lo < hq + hk && (keep || !a.seg[1].scatter))
-      head_run<T, NORM, HALF>(a, a.seg[1], tok, a.seg[1].scatter ? row : tok, max(lo, hq) - hq, min(hi, hq + hk) - hq,
-                              sub, u, slots, o0, o1, rotated, c, s, gain[1]);
-    if (hi > hq + hk && (keep || !a.seg[2].scatter))
-      head_run<T, NORM, HALF>(a, a.seg[2], tok, a.seg[2].scatter ? row : tok, max(lo, hq + hk) - hq - hk,
-                              hi - hq - hk, sub, u, slots, o0, o1, rotated, c, s, gain[1]);
+    if (lo < hq + hk)
+      head_run<T, NORM, HALF, G>(a, a.seg[1], tok, row, keep, max(lo, hq) - hq, min(hi, hq + hk) - hq, o0, o1, rotated, c,
+                                 s);
+    if (hi > hq + hk) head_copy<T, HALF>(a.seg[2], tok, row, keep, max(lo, hq + hk) - hq - hk, hi - hq - hk, o0, o1);
   }
 }
 
@@ -282,31 +315,52 @@ static int check_common(const char* who, long long tokens, int head_dim, int dty
   return LBW_OK;
 }
 
-template <typename T, bool NORM>
-static void launch_t(const HeadArgs& a, unsigned blocks, cudaStream_t s) {
-  if (a.rope.layout == LBW_ROPE_HALF)
-    head_rope_kernel<T, NORM, true><<<blocks, hr::THREADS, 0, s>>>(a);
+template <typename T, bool NORM, bool HALF>
+static void launch_g(const HeadArgs& a, int group, unsigned blocks, cudaStream_t s) {
+  if (group == 8)
+    head_rope_kernel<T, NORM, HALF, 8><<<blocks, hr::THREADS, 0, s>>>(a);
+  else if (group == 16)
+    head_rope_kernel<T, NORM, HALF, 16><<<blocks, hr::THREADS, 0, s>>>(a);
   else
-    head_rope_kernel<T, NORM, false><<<blocks, hr::THREADS, 0, s>>>(a);
+    head_rope_kernel<T, NORM, HALF, 32><<<blocks, hr::THREADS, 0, s>>>(a);
+}
+
+template <typename T, bool NORM>
+static void launch_t(const HeadArgs& a, int group, unsigned blocks, cudaStream_t s) {
+  if (a.rope.layout == LBW_ROPE_HALF)
+    launch_g<T, NORM, true>(a, group, blocks, s);
+  else
+    launch_g<T, NORM, false>(a, group, blocks, s);
 }
 
 template <bool NORM>
 static int launch_head_rope(HeadArgs& a, int dtype, cudaStream_t s, const char* who) {
   a.units = a.dim / 8;
-  a.group = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
+  const int group = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
   const int total = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
+  const long long most = (long long)num_sms() * hr::MINB;
+  const long long blocks_tok = (a.tokens + 32 / group - 1) / (32 / group);
+  // Heads per item: all of a token's, halved while the warps would have fewer than 8 items each (the last round is then
+  // a small part of the time), but not below 12, where the four angles of a lane (~240 instructions, a head is ~60) would
+  // weigh more than a third; below that only while there are fewer items than warps.
+  const long long warps = most * (hr::THREADS / 32);
   a.chunk = total;
-  a.chunks = 1;
-  const long long items = a.tokens * a.chunks;
+  while (a.chunk > hr::UN) {
+    const long long items = blocks_tok * ((total + a.chunk - 1) / a.chunk);
+    if (items >= (a.chunk > 12 ? 8 * warps : warps)) break;
+    a.chunk = (a.chunk + 1) / 2;
+  }
+  a.chunk = (a.chunk + hr::UN - 1) / hr::UN * hr::UN;
+  a.chunks = (total + a.chunk - 1) / a.chunk;
+  const long long items = blocks_tok * a.chunks;
   const long long want = (items + hr::THREADS / 32 - 1) / (hr::THREADS / 32);
-  const long long most = (long long)num_sms() * 8;
   const unsigned blocks = (unsigned)(want < most ? want : most);
   if (dtype == LBW_BF16)
-    launch_t<__nv_bfloat16, NORM>(a, blocks, s);
+    launch_t<__nv_bfloat16, NORM>(a, group, blocks, s);
   else if (dtype == LBW_FP16)
-    launch_t<__half, NORM>(a, blocks, s);
+    launch_t<__half, NORM>(a, group, blocks, s);
   else
-    launch_t<float, NORM>(a, blocks, s);
+    launch_t<float, NORM>(a, group, blocks, s);
   return cuda_check(cudaGetLastError(), who);
 }
 
@@ -323,7 +377,7 @@ int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, 
   if ((err = check_seg(who, "x", x, out, x_tok, x_head, out_tok, out_head, heads, dtype == LBW_FP32 ? 4 : 2)))
     return err;
   HeadArgs a{};
-  a.seg[0] = HeadSeg{x, out, nullptr, x_tok, x_head, out_tok, out_head, heads, 0, 0, 0};
+  a.seg[0] = HeadSeg{x, out, nullptr, x_tok, x_head, out_tok, out_head, heads, 0};
   a.tokens = tokens;
   a.dim = head_dim;
   a.pos = positions;
@@ -360,8 +414,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
       return err;
     if (r.gamma && !aligned(r.gamma, r.gamma_f32 ? 4 : 2))
       return set_error(LBW_ERR_ALIGN, "%s: gamma of %s is misaligned", who, names[i]);
-    a.seg[i] = HeadSeg{r.x,      r.out,   r.gamma,     r.x_tok, r.x_head, r.out_row,
-                       r.out_head, r.heads, r.gamma_f32, i == 2,  i > 0 && k_rows != nullptr};
+    a.seg[i] = HeadSeg{r.x, r.out, r.gamma, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads, r.gamma_f32};
   }
   a.tokens = tokens;
   a.dim = head_dim;

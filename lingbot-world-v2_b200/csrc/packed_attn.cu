@@ -116,6 +116,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     fence_mbar_init();
   }
   __syncthreads();
+  pdl_trigger();
   if (!found) return;  // the grid is an upper bound made from the row counts alone
   if (warp == 9) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
@@ -456,7 +457,11 @@ __global__ void __launch_bounds__(128) packed_merge_kernel(const __grid_constant
                                                            const __grid_constant__ TileArgs ta) {
   const int lane = threadIdx.x & 31;
   const long long wid = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (wid >= (long long)a.tq * a.hq) return;
+  if (wid >= (long long)a.tq * a.hq) {
+    pdl_wait();
+    return;
+  }
+  pdl_trigger();
   const long long tok = wid / a.hq;
   const int head = (int)(wid % a.hq);
   bool ours = false;
@@ -464,6 +469,7 @@ __global__ void __launch_bounds__(128) packed_merge_kernel(const __grid_constant
     const PackedSeq s = packed_seq(a, b);
     ours |= tok >= s.q0 && tok < s.q0 + s.nq && (long long)s.nq * a.group > ta.short_rows;
   }
+  pdl_wait();
   if (!__any_sync(0xffffffffu, ours)) return;
   const long long step = (long long)a.tq * a.hq;
   float M = -INFINITY;
@@ -508,8 +514,8 @@ static int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
   if ((err = cuda_check(cudaGetLastError(), "packed_attention launch"))) return err;
   if (ta.n_split > 1) {
     const long long rows = (long long)a.tq * a.hq;
-    packed_merge_kernel<D, F16><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a, ta);
-    err = cuda_check(cudaGetLastError(), "packed_attention merge launch");
+    err = launch_dependent("packed_attention merge launch", packed_merge_kernel<D, F16>, dim3((unsigned)((rows + 3) / 4)),
+                           128, 0, s, a, ta);
   }
   return err;
 }
@@ -546,12 +552,12 @@ struct PackedPlan {
   long long tile_floats, split_floats;  // workspace, fp32 values
 };
 
-static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, int n_seqs, int max_q) {
+static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, int n_seqs, int max_q, bool same_lens) {
   PackedPlan p{};
   const int group = hq / hk;
   const long long most = max_q > 0 && max_q < tq ? max_q : tq;
   p.tiles = most * group > SHORT_ROWS;
-  p.split = !p.tiles || n_seqs > 1;
+  p.split = !p.tiles || (n_seqs > 1 && !same_lens);  // (as many keys as queries: a short sequence is one tile)
   p.split_rows = p.tiles ? SHORT_ROWS : LLONG_MAX;  // (a sequence longer than max_q promised is still computed)
   if (p.split) p.split_floats = split_workspace_floats(d);
   if (!p.tiles) return p;
@@ -586,11 +592,11 @@ static int check_packed(long long tq, long long tk, int hq, int hk, int d, int n
 extern "C" {
 
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
-                                   long long* bytes, int* launches) {
+                                   int same_lens, long long* bytes, int* launches) {
   if (!bytes) return set_error(LBW_ERR_INVALID, "packed_attention_workspace: null pointer");
   const int err = check_packed(tq, tk, hq, hk, head_dim, n_seqs);
   if (err) return err;
-  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q);
+  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q, same_lens != 0);
   const bool any = tq > 0 && n_seqs > 0;
   *bytes = any ? (p.tile_floats + p.split_floats) * 4 : 0;
   if (launches) *launches = any ? (p.tiles ? 1 + (p.tile.n_split > 1) : 0) + (p.split ? 2 : 0) : 0;
@@ -612,7 +618,7 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   if (!q || !out || !cu_q || !cu_k || (tk > 0 && (!k || !v))) return set_error(LBW_ERR_INVALID, "%s: null pointer", who);
   if (!aligned(cu_q, 4) || !aligned(cu_k, 4) || !aligned(k_lens, 4) || !aligned(out, 16) || out_tok % 8 || out_head % 8)
     return set_error(LBW_ERR_ALIGN, "%s: the output needs a 16-byte aligned pointer and strides", who);
-  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q);
+  const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q, cu_q == cu_k && !k_lens);
   if (p.windows >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
   const long long need = (p.tile_floats + p.split_floats) * 4;
   if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
@@ -650,7 +656,7 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   if (!aligned(q, 16) || q_tok % 8 || q_head % 8)
     return set_error(LBW_ERR_ALIGN, "%s: q needs a 16-byte aligned pointer and strides", who);
   return launch_split(k, k_tok, k_head, v, v_tok, v_head, a, head_dim, dtype, q, q_tok, q_head, p.split_rows,
-                      ws + p.tile_floats, st, s);
+                      p.tiles, ws + p.tile_floats, st, s);
 }
 
 }  // extern "C"

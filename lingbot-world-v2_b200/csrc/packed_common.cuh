@@ -8,6 +8,12 @@
 
 namespace lbw {
 
+// Programmatic dependent launch between the kernels of one call: pdl_trigger lets the next kernel's blocks start as SMs
+// become free, pdl_wait holds a block until the kernels before it have finished and their writes are visible. Every
+// kernel that is launched this way waits before it ends, so what follows the call waits for all of them.
+LBW_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+LBW_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct PackedArgs {
   const int* cu_q;    // [n_seqs + 1] first query row of each sequence
   const int* cu_k;    // [n_seqs + 1] first key row

@@ -120,7 +120,11 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
       [&](longlong2 total) { return (long long)blockIdx.x * split_share(total.y, gridDim.x); }, tmp, &at_s);
   const long long share = split_share(at.total_y, gridDim.x);
   const long long first = blockIdx.x * share;
-  if (at.seq < 0 || at.sq.nk == 0) return;  // no tiles left for this CTA
+  pdl_trigger();
+  if (at.seq < 0 || at.sq.nk == 0) {  // no tiles left for this CTA
+    pdl_wait();
+    return;
+  }
   const long long last = min(first + share, at.total_y);
   const Abort ab{status, &abort_flag};
   SplitUnit u;
@@ -155,6 +159,7 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
       }
       for (int i = (j > STAGES ? j - STAGES : 0); i < j; ++i) mbar_wait_drain(&full[i % STAGES], (i / STAGES) & 1);
     }
+    pdl_wait();  // (it reads nothing of the kernels before it in the call: only its end comes after theirs)
     return;
   }
 
@@ -322,6 +327,7 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
     g += n;
     u = next_s;
   }
+  pdl_wait();
 }
 
 // Joins the units that crossed CTAs and writes the rows of sequences without keys. One block per unit.
@@ -334,6 +340,7 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
   const PackedAt at = packed_locate<128, false>(
       a, [&](int b) { return split_count(a, max_rows, b); }, [&](longlong2) { return (long long)blockIdx.x; }, tmp,
       &at_s);
+  pdl_wait();
   if (at.seq < 0) return;
   const PackedSeq sq = at.sq;
   const int n_tiles = (sq.nk + ps::KEYS - 1) / ps::KEYS;
@@ -372,7 +379,7 @@ long long split_workspace_floats(int d) { return 2ll * num_sms() * ps::ROWS * (d
 
 template <int D, bool F16>
 static int launch_split_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const PackedArgs& a, const void* q,
-                          long long q_tok, long long q_head, long long max_rows, float* ws, int* st, cudaStream_t s) {
+                          long long q_tok, long long q_head, long long max_rows, bool after, float* ws, int* st, cudaStream_t s) {
   static bool attr[64] = {};
   const int dix = device_index();
   if (dix < 0) return set_error(LBW_ERR_CUDA, "packed_attention: cudaGetDevice failed");
@@ -386,20 +393,27 @@ static int launch_split_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const 
   }
   const int ctas = num_sms();
   float* part_ml = ws + 2ll * ctas * ps::ROWS * D;
-  packed_split_kernel<D, F16><<<ctas, ps::THREADS, ps::smem_bytes(D), s>>>(
-      tmK, tmV, a, reinterpret_cast<const uint16_t*>(q), q_tok, q_head, max_rows, ws, part_ml, st);
-  if ((err = cuda_check(cudaGetLastError(), "packed_attention split launch"))) return err;
+  const uint16_t* q16 = reinterpret_cast<const uint16_t*>(q);
+  if (after) {
+    err = launch_dependent("packed_attention split launch", packed_split_kernel<D, F16>, dim3(ctas), ps::THREADS,
+                           ps::smem_bytes(D), s, tmK, tmV, a, q16, q_tok, q_head, max_rows, ws, part_ml, st);
+  } else {
+    packed_split_kernel<D, F16><<<ctas, ps::THREADS, ps::smem_bytes(D), s>>>(tmK, tmV, a, q16, q_tok, q_head, max_rows,
+                                                                            ws, part_ml, st);
+    err = cuda_check(cudaGetLastError(), "packed_attention split launch");
+  }
+  if (err) return err;
   // Row tiles: one per sequence of at most 16 rows; else at most one per sequence beyond tq * group / 16 full ones.
   const long long per_tok = (a.group + ps::ROWS - 1) / ps::ROWS;
   long long units = max_rows <= ps::ROWS ? a.n_seqs : (long long)a.tq * a.group / ps::ROWS + a.n_seqs;
   if (units > a.tq * per_tok) units = a.tq * per_tok;
-  packed_join_kernel<D, F16><<<(unsigned)(units * a.hk), 128, 0, s>>>(a, max_rows, ctas, ws, part_ml);
-  return cuda_check(cudaGetLastError(), "packed_attention join launch");
+  return launch_dependent("packed_attention join launch", packed_join_kernel<D, F16>, dim3((unsigned)(units * a.hk)), 128,
+                          0, s, a, max_rows, ctas, ws, part_ml);
 }
 
 int launch_split(const void* k, long long k_tok, long long k_head, const void* v, long long v_tok, long long v_head,
                  const PackedArgs& a, int d, int dtype, const void* q, long long q_tok, long long q_head,
-                 long long max_rows, float* ws, int* st, cudaStream_t s) {
+                 long long max_rows, bool after, float* ws, int* st, cudaStream_t s) {
   CUtensorMap tmK{}, tmV{};
   const CUtensorMapDataType ty = dtype == LBW_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   int err;
@@ -408,10 +422,10 @@ int launch_split(const void* k, long long k_tok, long long k_head, const void* v
     if ((err = make_tmap_3d(&tmV, v, ty, d, a.hk, a.tk, v_head, v_tok, 1, ps::KEYS))) return err;
   }
   if (d == 128)
-    return dtype == LBW_FP16 ? launch_split_t<128, true>(tmK, tmV, a, q, q_tok, q_head, max_rows, ws, st, s)
-                             : launch_split_t<128, false>(tmK, tmV, a, q, q_tok, q_head, max_rows, ws, st, s);
-  return dtype == LBW_FP16 ? launch_split_t<64, true>(tmK, tmV, a, q, q_tok, q_head, max_rows, ws, st, s)
-                           : launch_split_t<64, false>(tmK, tmV, a, q, q_tok, q_head, max_rows, ws, st, s);
+    return dtype == LBW_FP16 ? launch_split_t<128, true>(tmK, tmV, a, q, q_tok, q_head, max_rows, after, ws, st, s)
+                             : launch_split_t<128, false>(tmK, tmV, a, q, q_tok, q_head, max_rows, after, ws, st, s);
+  return dtype == LBW_FP16 ? launch_split_t<64, true>(tmK, tmV, a, q, q_tok, q_head, max_rows, after, ws, st, s)
+                           : launch_split_t<64, false>(tmK, tmV, a, q, q_tok, q_head, max_rows, after, ws, st, s);
 }
 
 }  // namespace lbw

@@ -900,21 +900,23 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
 
 
 @functools.lru_cache(4096)
-def _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, dev):
+def _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, same_lens, dev):
     """(workspace bytes, kernels launched) of a call with these sizes on device dev."""
     b, k = ctypes.c_longlong(0), ctypes.c_int(0)
     with torch.cuda.device(dev):
-        check(load().lbw_packed_attention_workspace(tq, tk, hq, hk, dim, n, max_q, ctypes.byref(b), ctypes.byref(k)),
+        check(load().lbw_packed_attention_workspace(tq, tk, hq, hk, dim, n, max_q, same_lens, ctypes.byref(b),
+                                                    ctypes.byref(k)),
               "packed_attention_workspace")
     return b.value, k.value
 
 
-def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=None):
+def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=None, same_lens=False):
     """Workspace (uint8) of packed_attention calls with these sizes, or None when they need none. Calls that may overlap
-    (other streams, graphs replayed side by side) need one each; packed_attention makes its own when given none."""
+    (other streams, graphs replayed side by side) need one each; packed_attention makes its own when given none.
+    same_lens: for calls with one tensor as cu_q and cu_k and no k_lens."""
     device = torch.device(device)
     dev = torch.cuda.current_device() if device.index is None else device.index
-    n, _ = _packed_attention_plan(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0), dev)
+    n, _ = _packed_attention_plan(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0), bool(same_lens), dev)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -957,7 +959,8 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
     if o_rows != tq or o_heads != hq:
         raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
-    ws_bytes, launches = _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, dev)
+    pq, pk = cu_q.data_ptr(), cu_k.data_ptr()
+    ws_bytes, launches = _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, pq == pk and k_lens is None, dev)
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError(f"{who}: the workspace must be contiguous")
@@ -967,7 +970,7 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
     with _on(dev):
         check(load().lbw_packed_attention(
             q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head, out.data_ptr(),
-            o_tok, o_head, cu_q.data_ptr(), cu_k.data_ptr(), None if k_lens is None else k_lens.data_ptr(), n, tq, tk,
-            hq, hk, dim, DTYPES[dtype], 1 if causal else 0, scale, max_q,
-            None if workspace is None else workspace.data_ptr(), ws_bytes, raw_stream(dev)), who, launches=launches)
+            o_tok, o_head, pq, pk, None if k_lens is None else k_lens.data_ptr(), n, tq, tk, hq, hk, dim, DTYPES[dtype],
+            1 if causal else 0, scale, max_q, None if workspace is None else workspace.data_ptr(), ws_bytes,
+            raw_stream(dev)), who, launches=launches)
     return out

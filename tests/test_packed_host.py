@@ -120,10 +120,10 @@ def test_packed_attention_entry_checks(lib, change, status):
 
 def test_packed_attention_refuses_a_small_workspace(lib):
     n = ctypes.c_longlong(-1)
-    assert lib.lbw_packed_attention_workspace(1, 100000, 8, 2, 128, 1, 1, ctypes.byref(n), None) == L.LBW_OK
+    assert lib.lbw_packed_attention_workspace(1, 100000, 8, 2, 128, 1, 1, 0, ctypes.byref(n), None) == L.LBW_OK
     assert n.value > 0
     rc = lib.lbw_packed_attention(P, 1024, 128, P, 1024, 128, P, 1024, 128, P, 1024, 128, P, P, None, 1, 1, 100000, 8, 2,
                                   128, 0, 1, 0.1, 1, P, n.value - 1, None)
     assert rc == L.LBW_ERR_INVALID and "workspace" in L.last_error()
-    assert lib.lbw_packed_attention_workspace(1, 100, 8, 3, 128, 1, 1, ctypes.byref(n), None) == L.LBW_ERR_SHAPE
-    assert lib.lbw_packed_attention_workspace(1, 100, 8, 2, 128, 1, 1, None, None) == L.LBW_ERR_INVALID
+    assert lib.lbw_packed_attention_workspace(1, 100, 8, 3, 128, 1, 1, 0, ctypes.byref(n), None) == L.LBW_ERR_SHAPE
+    assert lib.lbw_packed_attention_workspace(1, 100, 8, 2, 128, 1, 1, 0, None, None) == L.LBW_ERR_INVALID
