@@ -223,6 +223,11 @@ LBW_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
       LBW_W4(0), LBW_W4(4), LBW_W4(8), LBW_W4(12)
       : "memory");
 }
+LBW_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), LBW_W4(0),
+               LBW_W4(4)
+               : "memory");
+}
 LBW_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "

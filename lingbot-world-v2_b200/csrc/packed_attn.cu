@@ -8,14 +8,25 @@
 // the kv head's group sit side by side in a tile (row = token * pack + head), so that a tile of a short sequence is
 // filled by the group's heads. The two tiles are neighbours in the sequence; the "primary" is the later one, whose rows
 // see at least as many keys, and the secondary stops at its own last visible key tile.
-//   warps 0-3 / 4-7  softmax of the primary / secondary tile (thread = row = TMEM lane)
-//   warp 8           TMA producer: Q once, then K and V tiles through a 2-deep ring
-//   warp 9           UMMA issuer, TMEM owner (S0 | S1 | O0 | O1)
-//   warp 10          watches the K/V ring for the issuer (its arrivals fold "V(j) landed" and "K(j + 1) landed" into the
-//                    primary's two P barriers) and clears the value rows past the sequence's last key: they belong to
+//   warps 0-7 / 8-15 softmax of the primary / secondary tile, two threads per row (= TMEM lane): warps 0-3 and 8-11 have
+//                    the first 64 keys of a tile, 4-7 and 12-15 the others
+//   warp 16          TMA producer: Q once, then K and V tiles through a 2-deep ring
+//   warp 17          UMMA issuer, TMEM owner (S0 | S1 | O0 | O1)
+//   warp 19          scheduler: the CTA stays for many windows; while it works on one, this warp takes the next from the
+//                    blocks of the grid that have not started (cluster launch control) and works out its rows and keys,
+//                    so that the next Q, K and S are under way before the last rows of the present window are written
+//   warp 18          watches the K/V ring for the issuer (its arrival folds "V(j) and K(j + 1) landed" into the barrier that
+//                    announces the primary's P) and clears the value rows past the sequence's last key: they belong to
 //                    another sequence or to nobody, and 0 * NaN would reach the sum
-// The pipeline (P written over S in TMEM and released in two halves, a running maximum that moves only when it grows by
-// more than 2^8, a quarter of the exponentials on the FMA pipe) is the chunk attention's, see attn.cu for its figures.
+// P is written over S in TMEM, so a tile's chain is softmax, P V, next S; the two tiles take turns at the tensor pipe. The
+// running maximum moves only when it grows by more than 2^8.
+// What it measured (B200, D = 128, non-causal, cycles of one step = both tiles against 128 keys, 2,048 of them MMA at
+// full rate): 3,600, with the exponentials left out 3,600, with one tile's chain shortened by a third 3,500, with S or P V
+// left out 2,550, with all MMAs left out 1,470: the MMAs of a tile and the hand-overs around them (commit, softmax warps,
+// arrival, issuer: ~600 cycles without any work in between) follow each other, and the exponentials hide behind the other
+// tile. Tried and slower: exponentials on the FMA pipe (1/8 to 1/2 of them, +1 to +5%), an issuer per tile (+4 to +20%),
+// one thread per row and two P releases (+10%), P beside S for D = 64 (-8% for long sequences, +10% for short ones), the
+// maximum of the tile before as m (+5%), rolled MMA loops (+8%), waits of one lane (+17%) or with a suspend hint (+7%).
 // Rows that see no key (causal with fewer keys than queries, no keys at all) get zeros.
 #include <limits.h>
 
@@ -28,8 +39,10 @@ namespace lbw {
 namespace pa {
 constexpr int BM = 128, BN = 128, STAGES = 2;
 constexpr int HALF = 128 * 64 * 2;  // 128 rows x 64 16-bit values: one 128-byte swizzled box
-constexpr int THREADS = 352;
-constexpr int smem_bytes(int d) { return (2 + 2 * STAGES) * (d / 64) * HALF + 1024; }
+constexpr int SOFT_WARPS = 16;  // warps 0-15: (tile, key half) = (warp / 8, warp / 4 % 2), rows by warp % 4
+constexpr int THREADS = (SOFT_WARPS + 4) * 32;
+constexpr int STAGE_BYTES = SOFT_WARPS * 2048;  // output staging: 32 rows x 32 columns for each softmax warp
+constexpr int smem_bytes(int d) { return (2 + 2 * STAGES) * (d / 64) * HALF + STAGE_BYTES + 1024; }
 }  // namespace pa
 
 struct TileArgs {
@@ -42,23 +55,85 @@ struct TileArgs {
   float* part_ml;  // [n_split][tq * hq][2]
 };
 
-// Two 2^x on the FMA pipe (see exp2_poly2), NaN kept.
-LBW_DEV void exp2_poly2_nan(float x0, float x1, float& y0, float& y1) {
-  float a, b;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(x0), "f"(-126.f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(x1), "f"(-126.f));
-  const uint64_t x = f2_pack(a, b);
-  const uint64_t t = f2_add(x, f2_pack(12582912.f, 12582912.f));
-  const uint64_t n = f2_add(t, f2_pack(-12582912.f, -12582912.f));
-  const uint64_t f = f2_fma(n, f2_pack(-1.f, -1.f), x);
-  uint64_t p = f2_fma(f2_pack(0.054602623f, 0.054602623f), f, f2_pack(0.24192412f, 0.24192412f));
-  p = f2_fma(p, f, f2_pack(0.69331646f, 0.69331646f));
-  p = f2_fma(p, f, f2_pack(1.f, 1.f));
-  float p0, p1, t0, t1;
-  f2_unpack(p, p0, p1);
-  f2_unpack(t, t0, t1);
-  y0 = __int_as_float(__float_as_int(p0) + ((__float_as_int(t0) - 0x4B400000) << 23));
-  y1 = __int_as_float(__float_as_int(p1) + ((__float_as_int(t1) - 0x4B400000) << 23));
+// tcgen05 operations of a converged warp, issued by the lanes with lead != 0 (one of them).
+LBW_DEV void mma_f16_ss_if(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+LBW_DEV void mma_f16_ts_if(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+LBW_DEV void tc_commit_if(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
+// One window: the key range [g0, g0 + n_p) (in 128-key tiles) of a pair of query tiles.
+struct PackedWin {
+  PackedSeq sq;
+  int tok[2];   // first token of the primary and of the secondary tile
+  int n_p, n_s; // key tiles of the primary; the secondary takes the first n_s of them
+  int g0, split, head0, two;
+  int valid;
+};
+
+// Next window of the grid, for the block that calls it: takes the place of a block that has not been launched yet
+// (cluster launch control). The answer arrives in `res` with 16 bytes on `bar`.
+LBW_DEV void steal_request(void* res, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(res)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+LBW_DEV bool steal_answer(const void* res, unsigned& block) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}\n"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(res))
+      : "memory");
+  block = x;
+  return ok != 0;
+}
+
+// mbar_arrive of the lanes with lead != 0.
+LBW_DEV void mbar_arrive_if(uint32_t lead, uint64_t* bar) {
+  asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}\n" ::"r"(
+                   smem_u32(bar)),
+               "r"(lead)
+               : "memory");
+}
+
+// The two warps of one group of rows meet (barrier `id`, 64 threads); pair_all: whether `ok` holds for all of them.
+LBW_DEV void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+LBW_DEV bool pair_all(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(id), "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
 }
 
 template <int D, bool F16>
@@ -74,31 +149,18 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
   uint8_t* sQ = smem;
   uint8_t* sK = smem + 2 * TILE;
   uint8_t* sV = sK + STAGES * TILE;
-  __shared__ __align__(8) uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2],
-      p_ready[2][2], o_done[2], done_bar;
+  uint8_t* s_stage = sV + STAGES * TILE;
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES],
+      s_full[2], p_ready[2], o_done[2], win_full[2], win_empty[2], want_next, steal_bar, done_bar;
+  __shared__ __align__(16) uint4 steal_res;
+  __shared__ PackedWin s_win[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ int found;
-  __shared__ PackedSeq found_seq;
-  __shared__ int found_item;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    int b = -1;
-    long long l = 0;
-    const bool ok = packed_find(a.n_seqs, (long long)(blockIdx.x / ta.head_tiles), [&](int i) {
-      const PackedSeq s = packed_seq(a, i);
-      if ((long long)s.nq * a.group <= ta.short_rows) return 0;
-      return (s.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
-    }, b, l);
-    if (lane == 0) {
-      found = ok;
-      found_item = (int)l;
-      if (ok) found_seq = packed_seq(a, b);
-    }
-  }
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -107,307 +169,415 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i][0], 128 + (i == 0));  // P of keys 0..63 written (+ V(j) landed, for the primary)
-      mbar_init(&p_ready[i][1], 128 + (i == 0));  // P of keys 64..127 written (+ K(j + 1) landed, for the primary)
+      mbar_init(&p_ready[i], 8 + (i == 0));  // P written by 8 warps (+ V(j) and K(j + 1) landed, for the primary)
       mbar_init(&o_done[i], 1);
+      mbar_init(&win_full[i], 1);
+      mbar_init(&win_empty[i], 3 + SOFT_WARPS);  // producer, issuer, watcher and the softmax warps have read the window
     }
+    mbar_init(&want_next, 1);
+    mbar_init(&steal_bar, 1);
     mbar_init(&done_bar, 1);
     abort_flag = 0;
     fence_mbar_init();
   }
-  __syncthreads();
-  pdl_trigger();
-  if (!found) return;  // the grid is an upper bound made from the row counts alone
-  if (warp == 9) tmem_alloc(&tmem_slot, 512);
+  if (warp == 17) tmem_alloc(&tmem_slot, 512);
+  // Rows that no token fills (pack does not divide 128): zeros, so that they never ask for a rescale.
+  const int filled = ta.pack * ta.tile_toks;
+  for (int e = filled * 8 + threadIdx.x; e < 128 * 8; e += THREADS)
+    for (int t = 0; t < 2 * NH; ++t) *reinterpret_cast<uint4*>(sQ + t * HALF + e * 16) = make_uint4(0, 0, 0, 0);
+  fence_async_shared();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();
   const uint32_t tmem = tmem_slot;
   const Abort ab{status, &abort_flag};
 
-  // The window: pairs of tiles of a sequence are taken from its end, where causal rows see most keys.
-  const PackedSeq sq = found_seq;
-  const int n_pairs = (sq.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
-  const int tok0 = (n_pairs - 1 - found_item) * 2 * ta.tile_toks;
-  const bool two = tok0 + ta.tile_toks < sq.nq;
-  const int head0 = (int)(blockIdx.x % ta.head_tiles) * ta.pack;
-  const int kv_head = head0 / a.group;
-  int tile_tok[2];  // first token of the primary and of the secondary tile
-  tile_tok[0] = two ? tok0 + ta.tile_toks : tok0;
-  tile_tok[1] = tok0;
-  const int keys_p = packed_visible(a, sq, min(tile_tok[0] + ta.tile_toks, sq.nq) - 1);
-  const int keys_s = two ? packed_visible(a, sq, tok0 + ta.tile_toks - 1) : 0;
-  const int all_p = (keys_p + BN - 1) / BN, all_s = (keys_s + BN - 1) / BN;
-  // This CTA's key tiles [g0, g0 + n_p); the secondary takes the first n_s of them.
-  const int g0 = (int)((long long)blockIdx.y * all_p / ta.n_split);
-  const int n_p = (int)((long long)(blockIdx.y + 1) * all_p / ta.n_split) - g0;
-  const int n_s = min(max(all_s - g0, 0), n_p);
-
-  if (warp == 8) {
-    // ---------------- producer ----------------
-    if (lane == 0 && n_p > 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      mbar_expect_tx(&q_full, (n_s > 0 ? 2 : 1) * NH * ta.pack * ta.tile_toks * 128);
-      for (int i = 0; i < (n_s > 0 ? 2 : 1); ++i)
-        for (int h = 0; h < NH; ++h)
-          tma_load_3d(sQ + i * TILE + h * HALF, &tmQ, &q_full, h * 64, head0, sq.q0 + tile_tok[i]);
-      int j = 0;
-      for (; j < n_p; ++j) {
-        const int s = j & 1;
-        const uint32_t ph = (j >> 1) & 1;
-        const int row = sq.k0 + (g0 + j) * BN;
-        if (!mbar_wait(&k_empty[s], ph ^ 1, ab, 0x21)) break;
-        mbar_expect_tx(&k_full[s], TILE);
-        for (int h = 0; h < NH; ++h) tma_load_3d(sK + s * TILE + h * HALF, &tmK, &k_full[s], h * 64, kv_head, row);
-        if (!mbar_wait(&v_empty[s], ph ^ 1, ab, 0x22)) {
-          mbar_wait_drain(&k_full[s], ph);
-          break;
-        }
-        mbar_expect_tx(&v_full[s], TILE);
-        for (int h = 0; h < NH; ++h) tma_load_3d(sV + s * TILE + h * HALF, &tmV, &v_full[s], h * 64, kv_head, row);
-      }
-      // Let the last loads of each ring slot land before the CTA can exit.
-      mbar_wait_drain(&q_full, 0);
-      for (int i = (j > STAGES ? j - STAGES : 0); i < j; ++i) {
-        mbar_wait_drain(&k_full[i & 1], (i >> 1) & 1);
-        mbar_wait_drain(&v_full[i & 1], (i >> 1) & 1);
-      }
-    }
-  } else if (warp == 9) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0 && n_p > 0) {
-      const uint32_t idesc_s = F16 ? idesc_f16(BM, BN, 0, 0) : idesc_bf16(BM, BN, 0, 0);  // S = Q K^T, both K-major
-      const uint32_t idesc_o = F16 ? idesc_f16(BM, D, 0, 1) : idesc_bf16(BM, D, 0, 1);    // O += P V, V MN-major
-      const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
-      const uint64_t dK = sdesc_kmajor_sw128(smem_u32(sK));
-      const uint64_t dV = sdesc_mnmajor_sw128(smem_u32(sV), HALF);
-      auto issue_s = [&](int i, int stage) {
-        const uint64_t q = dQ + (uint64_t)((i * TILE) >> 4), k = dK + (uint64_t)((stage * TILE) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
-          mma_f16_ss(tmem + i * 128, q + off, k + off, idesc_s, kk > 0);
-        }
-      };
-      auto issue_pv = [&](int i, int stage, bool first, int half) {  // keys 0..63 (half 0) or 64..127
-        const uint64_t v = dV + (uint64_t)((stage * TILE) >> 4);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int kk = half * 4 + q;
-          mma_f16_ts(tmem + 256 + i * D, tmem + i * 128 + kk * 8, v + (uint64_t)((kk * 2048) >> 4), idesc_o,
-                     !(first && kk == 0));
-        }
-      };
-      bool ok = mbar_wait(&q_full, 0, ab, 0x31) && mbar_wait(&k_full[0], 0, ab, 0x32);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0, 0);
-        tc_commit(&s_full[0]);
-        if (n_s > 0) {
-          issue_s(1, 0);
-          tc_commit(&s_full[1]);
-        }
-        tc_commit(&k_empty[0]);
-        for (int j = 0; j < n_p; ++j) {
-          const int s = j & 1, s1 = (j + 1) & 1;
-          const bool more = j + 1 < n_p;
-          if (!mbar_wait(&p_ready[0][0], j & 1, ab, 0x34)) break;
-          tc_fence_after();
-          issue_pv(0, s, j == 0, 0);
-          if (!mbar_wait(&p_ready[0][1], j & 1, ab, 0x37)) break;
-          tc_fence_after();
-          issue_pv(0, s, j == 0, 1);
-          if (more) {
-            issue_s(0, s1);
-            tc_commit(&s_full[0]);
-          } else {
-            tc_commit(&o_done[0]);
+  if (warp == 19) {
+    // ---------------- scheduler ----------------
+    // Takes the next window when the producer loads the last key tile of the present one: about two tiles before its end,
+    // enough to hide the answer and the search, and late enough that no CTA holds work which another could start.
+    // Windows come in the grid's order, so the search for a window's sequence goes on where the last one ended.
+    bool have = true;
+    unsigned block = blockIdx.x;
+    int b_at = 0, loaded = -1;
+    unsigned before = 0;  // windows of the sequences before b_at (all counts are below the grid's 2^31)
+    PackedSeq s{0, 0, 0, 0};
+    unsigned own = 0, upto = 0;
+    for (int i = 0;; ++i) {
+      const int slot = i & 1;
+      bool ok = true;
+      if (i > 0) {
+        if (lane == 0) {
+          ok = mbar_wait_c(&want_next, (i - 1) & 1, ab, 0x13);
+          if (ok) {
+            mbar_expect_tx(&steal_bar, 16);
+            steal_request(&steal_res, &steal_bar);
+            ok = mbar_wait_c(&steal_bar, (i - 1) & 1, ab, 0x11);
           }
-          if (j < n_s) {
-            if (!mbar_wait(&p_ready[1][0], j & 1, ab, 0x36)) break;
-            tc_fence_after();
-            issue_pv(1, s, j == 0, 0);
-            if (!mbar_wait(&p_ready[1][1], j & 1, ab, 0x38)) break;
-            tc_fence_after();
-            issue_pv(1, s, j == 0, 1);
-          }
-          tc_commit(&v_empty[s]);
-          if (j + 1 < n_s) {
-            issue_s(1, s1);
-            tc_commit(&s_full[1]);
-          } else if (j + 1 == n_s) {
-            tc_commit(&o_done[1]);
-          }
-          if (more) tc_commit(&k_empty[s1]);
+          have = ok && steal_answer(&steal_res, block);
+          fence_async_shared();  // (read before the next answer overwrites it)
         }
+        have = __shfl_sync(0xffffffffu, have, 0);
+        block = __shfl_sync(0xffffffffu, block, 0);
       }
-      tc_commit(&done_bar);
-      mbar_wait_drain(&done_bar, 0);
-    }
-  } else if (warp == 10) {
-    // ---------------- K/V watcher ----------------
-    // In landing order, one phase of each P barrier at a time (see attn.cu).
-    bool ok = n_p > 0;
-    if (ok && lane == 0) ok = mbar_wait(&k_full[0], 0, ab, 0x60);
-    ok = __shfl_sync(0xffffffffu, ok, 0);
-    for (int j = 0; j < n_p && ok; ++j) {
-      const int s = j & 1;
-      if (lane == 0) ok = mbar_wait(&v_full[s], (j >> 1) & 1, ab, 0x61);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
-      const int rows = sq.nk - (g0 + j) * BN;  // value rows of this tile that are the sequence's
-      if (rows < BN) {
-        for (int i = rows * 8 + lane; i < BN * 8; i += 32)
+      PackedWin w;
+      w.valid = 0;
+      if (have) {
+        const unsigned rest = ta.n_split > 1 ? block / ta.n_split : block;
+        w.split = (int)(block - rest * ta.n_split);
+        const unsigned pair = rest / ta.head_tiles;
+        w.head0 = (int)(rest - pair * ta.head_tiles) * ta.pack;
+        while (b_at < a.n_seqs) {
+          if (loaded != b_at) {  // 32 sequences, one per lane, kept while windows come from them
+            const int b = b_at + lane;
+            s = b < a.n_seqs ? packed_seq(a, b) : PackedSeq{0, 0, 0, 0};
+            own = (long long)s.nq * a.group <= ta.short_rows ? 0 : (s.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
+            upto = own;
 #pragma unroll
-          for (int h = 0; h < NH; ++h)
-            *reinterpret_cast<uint4*>(sV + s * TILE + h * HALF + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_async_shared();
-        __syncwarp();
+            for (int o = 1; o < 32; o <<= 1) {
+              const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+              if (lane >= o) upto += v;
+            }
+            loaded = b_at;
+          }
+          const unsigned hit = __ballot_sync(0xffffffffu, before + upto > pair);
+          if (hit) {
+            const int at = __ffs(hit) - 1;
+            w.valid = 1;
+            w.sq.q0 = __shfl_sync(0xffffffffu, s.q0, at);
+            w.sq.nq = __shfl_sync(0xffffffffu, s.nq, at);
+            w.sq.k0 = __shfl_sync(0xffffffffu, s.k0, at);
+            w.sq.nk = __shfl_sync(0xffffffffu, s.nk, at);
+            // Pairs of tiles are taken from the sequence's end, where causal rows see most keys. (The minimum is for starts
+            // that overlap so often that the counts wrap.)
+            const unsigned n_pairs = __shfl_sync(0xffffffffu, own, at);
+            const unsigned l = min(pair - before - __shfl_sync(0xffffffffu, upto - own, at), n_pairs - 1);
+            const int tok0 = (int)(n_pairs - 1 - l) * 2 * ta.tile_toks;
+            w.two = tok0 + ta.tile_toks < w.sq.nq;
+            w.tok[0] = w.two ? tok0 + ta.tile_toks : tok0;
+            w.tok[1] = tok0;
+            const int keys_p = packed_visible(a, w.sq, min(w.tok[0] + ta.tile_toks, w.sq.nq) - 1);
+            const int keys_s = w.two ? packed_visible(a, w.sq, tok0 + ta.tile_toks - 1) : 0;
+            const int all_p = (keys_p + BN - 1) / BN, all_s = (keys_s + BN - 1) / BN;
+            w.g0 = 0;
+            w.n_p = all_p;
+            if (ta.n_split > 1) {  // (n_split <= 16 and all_p < 2^24: no overflow)
+              w.g0 = w.split * all_p / ta.n_split;
+              w.n_p = (w.split + 1) * all_p / ta.n_split - w.g0;
+            }
+            w.n_s = min(max(all_s - w.g0, 0), w.n_p);
+            break;
+          }
+          before += __shfl_sync(0xffffffffu, upto, 31);
+          b_at += 32;
+        }
       }
       if (lane == 0) {
-        mbar_arrive(&p_ready[0][0]);
-        ok = j + 1 >= n_p || mbar_wait(&k_full[s ^ 1], ((j + 1) >> 1) & 1, ab, 0x62);
-        if (ok) {
-          mbar_arrive(&p_ready[0][1]);
-          ok = mbar_wait(&p_ready[0][0], j & 1, ab, 0x63) && mbar_wait(&p_ready[0][1], j & 1, ab, 0x64);
-        }
+        ok = mbar_wait_c(&win_empty[slot], ((i >> 1) & 1) ^ 1, ab, 0x10) && ok;
+        s_win[slot] = w;
+        mbar_arrive(&win_full[slot]);
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!w.valid || !ok) {
+        // Past the last window (the grid is an upper bound): take the blocks that are left, so that none has to start.
+        for (int t = i; lane == 0 && have && ok; ++t) {
+          mbar_expect_tx(&steal_bar, 16);
+          steal_request(&steal_res, &steal_bar);
+          if (!mbar_wait_c(&steal_bar, t & 1, ab, 0x12)) break;
+          have = steal_answer(&steal_res, block);
+          fence_async_shared();
+        }
+        break;
+      }
+    }
+  } else if (warp == 16) {
+    // ---------------- producer ----------------
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      int j = 0, nq_loads = 0;  // K/V tiles and Q pairs loaded so far
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        if (!mbar_wait_c(&win_full[i & 1], (i >> 1) & 1, ab, 0x20)) break;
+        const PackedWin w = s_win[i & 1];
+        mbar_arrive(&win_empty[i & 1]);
+        if (!w.valid) break;
+        const int kv_head = w.head0 / a.group;
+        if (w.n_p == 0) mbar_arrive(&want_next);
+        for (int t = 0; t < w.n_p; ++t, ++j) {
+          if (t + 1 == w.n_p) mbar_arrive(&want_next);
+          const int s = j & 1;
+          const uint32_t ph = (j >> 1) & 1;
+          const int row = w.sq.k0 + (w.g0 + t) * BN;
+          if (!(ok = mbar_wait_c(&k_empty[s], ph ^ 1, ab, 0x21))) break;
+          mbar_expect_tx(&k_full[s], TILE);
+          for (int h = 0; h < NH; ++h) tma_load_3d(sK + s * TILE + h * HALF, &tmK, &k_full[s], h * 64, kv_head, row);
+          if (t == 0) {  // the pair's Q goes where the last window's was, once its last S is computed
+            if (!(ok = mbar_wait_c(&q_empty, (nq_loads & 1) ^ 1, ab, 0x23))) { mbar_wait_drain(&k_full[s], ph); break; }
+            const int tiles = w.n_s > 0 ? 2 : 1;
+            mbar_expect_tx(&q_full, tiles * NH * ta.pack * ta.tile_toks * 128);
+            for (int q = 0; q < tiles; ++q)
+              for (int h = 0; h < NH; ++h)
+                tma_load_3d(sQ + q * TILE + h * HALF, &tmQ, &q_full, h * 64, w.head0, w.sq.q0 + w.tok[q]);
+            ++nq_loads;
+          }
+          if (!(ok = mbar_wait_c(&v_empty[s], ph ^ 1, ab, 0x22))) { mbar_wait_drain(&k_full[s], ph); break; }
+          mbar_expect_tx(&v_full[s], TILE);
+          for (int h = 0; h < NH; ++h) tma_load_3d(sV + s * TILE + h * HALF, &tmV, &v_full[s], h * 64, kv_head, row);
+        }
+      }
+      // Let the last loads of each ring slot land before the CTA can exit.
+      if (nq_loads > 0) mbar_wait_drain(&q_full, (nq_loads - 1) & 1);
+      for (int t = (j > STAGES ? j - STAGES : 0); t < j; ++t) {
+        mbar_wait_drain(&k_full[t & 1], (t >> 1) & 1);
+        mbar_wait_drain(&v_full[t & 1], (t >> 1) & 1);
+      }
+    }
+  } else if (warp == 17) {
+    // ---------------- MMA issuer ----------------
+    // MMAs execute in issue order: S of a window's first tile may be issued right behind the last P V of the window
+    // before, and its O is overwritten only by a P V that waits for a P written after that O was read.
+    // The whole warp runs this code and lane 0 issues (by predicate): in a branch of one lane every descriptor would have to
+    // be moved to the uniform registers that the MMA reads.
+    const uint32_t lead = lane == 0;
+    const uint32_t idesc_s = F16 ? idesc_f16(BM, BN, 0, 0) : idesc_bf16(BM, BN, 0, 0);  // S = Q K^T, both K-major
+    const uint32_t idesc_o = F16 ? idesc_f16(BM, D, 0, 1) : idesc_bf16(BM, D, 0, 1);    // O += P V, V MN-major
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const uint64_t dQ = sdesc_kmajor_sw128(smem_u32(sQ));
+    const uint64_t dK = sdesc_kmajor_sw128(smem_u32(sK));
+    const uint64_t dV = sdesc_mnmajor_sw128(smem_u32(sV), HALF);
+    auto issue_s = [&](int i, int stage) {
+      const uint64_t q = dQ + (uint64_t)((i * TILE) >> 4), k = dK + (uint64_t)((stage * TILE) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
+        mma_f16_ss_if(lead, tm + i * 128, q + off, k + off, idesc_s, kk > 0);
+      }
+    };
+    auto issue_pv = [&](int i, int stage, bool first) {
+      const uint64_t v = dV + (uint64_t)((stage * TILE) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)  // P of keys 64.. lies over its own scores, 64 columns on
+        mma_f16_ts_if(lead, tm + 256 + i * D, tm + i * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+                      v + (uint64_t)((kk * 2048) >> 4), idesc_o, !(first && kk == 0));
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+      return __all_sync(0xffffffffu, mbar_wait_c(bar, parity, ab, site)) != 0;
+    };
+    int jp = 0, js = 0, nq_loads = 0;  // tiles of the primaries and secondaries, Q pairs, so far
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!wait(&win_full[i & 1], (i >> 1) & 1, 0x30)) break;
+      const int n_p = __shfl_sync(0xffffffffu, s_win[i & 1].n_p, 0), n_s = __shfl_sync(0xffffffffu, s_win[i & 1].n_s, 0);
+      const int valid = __shfl_sync(0xffffffffu, s_win[i & 1].valid, 0);
+      if (lead) mbar_arrive(&win_empty[i & 1]);
+      if (!valid) break;
+      if (n_p == 0) continue;
+      if (!wait(&q_full, nq_loads & 1, 0x31) || !wait(&k_full[jp & 1], (jp >> 1) & 1, 0x32)) break;
+      ++nq_loads;
+      tc_fence_after();
+      // Step j: P V of tile j, then S of tile j + 1 (step -1 has only the first S): the same code for all steps, so that
+      // it is in the instruction cache when a window begins.
+      for (int j = -1; ok && j < n_p; ++j) {
+        const int s = jp & 1, s1 = j < 0 ? s : s ^ 1;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int n = t ? n_s : n_p;
+          if (t && j >= 0 && (j >= n || !ok)) tc_commit_if(lead, &v_empty[s]);
+          if (j >= n || !ok) continue;
+          if (j >= 0) {
+            if (!(ok = wait(&p_ready[t], (t ? js : jp) & 1, 0x34 + t))) continue;
+            tc_fence_after();
+            issue_pv(t, s, j == 0);
+            js += t;
+            if (t) tc_commit_if(lead, &v_empty[s]);
+          }
+          if (j + 1 < n) {
+            issue_s(t, s1);
+            tc_commit_if(lead, &s_full[t]);
+          } else if (n > 0) {
+            tc_commit_if(lead, &o_done[t]);
+          }
+        }
+        if (j + 1 < n_p) tc_commit_if(lead, &k_empty[s1]);
+        if (j + 2 == n_p) tc_commit_if(lead, &q_empty);  // the window's last S has been issued
+        jp += j >= 0;
+      }
+    }
+    tc_commit_if(lead, &done_bar);
+    mbar_wait_drain(&done_bar, 0);
+  } else if (warp == 18) {
+    // ---------------- K/V watcher ----------------
+    // One phase of each P barrier at a time (see attn.cu). It must never wait for a phase that can be lapped: it does not
+    // look at a window's first K, whose S and whose slot's next load (K two tiles on) do not depend on it, so that two
+    // phases could pass before it looked. Every K and V that it waits for is followed by its own arrival before the
+    // slot can be loaded again, and the phase before it is over: its S or P V was needed for the P seen before.
+    int jp = 0;
+    // All lanes wait: a wait of one lane of a converged warp costs ~500 cycles more (a round trip of two warps over mbarriers
+    // takes 290 cycles when all lanes wait, 1,220 when lane 0 waits for the others), and these are on every tile's path.
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait_c(&win_full[i & 1], (i >> 1) & 1, ab, 0x5f))) break;
+      const int n_p = s_win[i & 1].n_p, left = s_win[i & 1].sq.nk - s_win[i & 1].g0 * BN, valid = s_win[i & 1].valid;
+      __syncwarp();
+      mbar_arrive_if(lane == 0, &win_empty[i & 1]);
+      if (!valid) break;
+      for (int j = 0; j < n_p; ++j, ++jp) {
+        const int s = jp & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_c(&v_full[s], (jp >> 1) & 1, ab, 0x61));
+        if (!ok) break;
+        const int rows = left - j * BN;  // value rows of this tile that are the sequence's
+        if (rows < BN) {
+          for (int r = rows * 8 + lane; r < BN * 8; r += 32)
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+              *reinterpret_cast<uint4*>(sV + s * TILE + h * HALF + r * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_shared();
+          __syncwarp();
+        }
+        ok = j + 1 >= n_p || __all_sync(0xffffffffu, mbar_wait_c(&k_full[s ^ 1], ((jp + 1) >> 1) & 1, ab, 0x62));
+        if (!ok) break;
+        mbar_arrive_if(lane == 0, &p_ready[0]);
+        ok = __all_sync(0xffffffffu, mbar_wait_c(&p_ready[0], jp & 1, ab, 0x63));
+        if (!ok) break;
+      }
     }
   } else {
     // ---------------- softmax / correction / epilogue ----------------
-    const int wg = warp >> 2;
+    // Two threads per row, one for each half of a tile's keys, in two warps that meet at a named barrier for the row's
+    // maximum. They take every branch together: their row values are equal, and they agree on the waits (a warp that
+    // left alone would leave the other at the barrier).
+    const int wg = warp >> 3, half = (warp >> 2) & 1;
     const int r0 = (warp & 3) * 32 + lane;  // row of the tile
+    const int pair_bar = 1 + wg * 4 + (warp & 3);
+    uint8_t* stage = s_stage + warp * 2048;  // this warp's 2 KB: its rows' maxima and sums, and the output on its way
+    float* my_row = reinterpret_cast<float*>(stage) + lane;
+    const float* other_row = reinterpret_cast<const float*>(s_stage + (warp ^ 4) * 2048) + lane;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + lane_off + wg * 128;
-    const uint32_t tO = tmem + lane_off + 256 + wg * D;
-    const int tok = tile_tok[wg] + r0 / ta.pack;
-    const bool mine = (wg == 0 || two) && r0 < ta.pack * ta.tile_toks && tok < sq.nq;
-    const int seen = mine ? packed_visible(a, sq, tok) - g0 * BN : 0;  // keys this row sees, from this CTA's first on
-    const int n_tiles = wg == 0 ? n_p : n_s;
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int j = 0; j < n_tiles; ++j) {
-      const int valid = seen - j * BN;
-      if (!mbar_wait(&s_full[wg], j & 1, ab, 0x40 + wg)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t r[128];
-      tmem_ld32(tS + 0, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-      tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
-      tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&r[64]));
-      tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&r[96]));
-      tmem_ld_wait();
-      float* sv = reinterpret_cast<float*>(r);
-      const bool whole = __all_sync(0xffffffffu, valid >= BN || !mine);
-      if (!whole) {  // the diagonal, or the sequence's last tile
-#pragma unroll
-        for (int e = 0; e < BN; ++e)
-          if (e >= valid) sv[e] = -INFINITY;
+    const uint32_t tS = tmem + lane_off + wg * 128 + half * 64;
+    const uint32_t tO = tmem + lane_off + 256 + wg * D + half * (D / 2);  // this thread's columns of O
+    uint32_t phases = 0;  // bit 0: parity of s_full (tiles so far), bit 1: of o_done (windows with a tile)
+    for (int i = 0;; ++i) {
+      const bool got = mbar_wait_c(&win_full[i & 1], (i >> 1) & 1, ab, 0x40);
+      if (!pair_all(pair_bar, got && !abort_flag)) break;
+      const volatile PackedWin& w = s_win[i & 1];  // read again at the end: registers are short in between
+      if (!w.valid) break;
+      if (wg == 1 && !w.two) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&win_empty[i & 1]);
+        continue;
       }
-      float t8[8];
+      // Keys this row sees, from this thread's first on; a row that is nobody's is never masked (nor written).
+      int seen = 1 << 30;
+      {
+        const int nq = w.sq.nq, nk = w.sq.nk, tok = w.tok[wg] + r0 / ta.pack;
+        if (r0 < ta.pack * ta.tile_toks && tok < nq)
+          seen = packed_visible(a, PackedSeq{0, nq, 0, nk}, tok) - w.g0 * BN - half * 64;
+      }
+      const int n_tiles = wg == 0 ? w.n_p : w.n_s;
+      float m = -INFINITY, l = 0.f;
+      for (int left = n_tiles; left > 0; --left, seen -= BN, phases ^= 1) {
+        mbar_wait_c(&s_full[wg], phases & 1, ab, 0x41 + wg);  // (after a timeout the window runs on, and ends the loop)
+        tc_fence_after();
+        uint32_t r[64];
+        float* sv = reinterpret_cast<float*>(r);
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        tmem_ld_wait();
+        if (!__all_sync(0xffffffffu, seen >= 64)) {  // the diagonal, or the sequence's last tile
 #pragma unroll
-      for (int q = 0; q < 8; ++q) t8[q] = sv[q];
+          for (int cc = 0; cc < 2; ++cc) {
+            const int n = min(max(seen - cc * 32, 0), 32);
+            const uint32_t keep = n == 32 ? 0xffffffffu : (1u << n) - 1u;
 #pragma unroll
-      for (int e = 8; e < 120; e += 16)
-#pragma unroll
-        for (int q = 0; q < 8; ++q) t8[q] = fmax3(t8[q], sv[e + q], sv[e + 8 + q]);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) t8[q] = fmaxf(t8[q], sv[120 + q]);
-      const float mx =
-          fmaxf(fmax3(t8[0], t8[1], t8[2]), fmax3(fmax3(t8[3], t8[4], t8[5]), t8[6], t8[7])) * a.scale_log2;
-      const float m_new = fmaxf(m, mx);
-      float alpha = 1.f;
-      bool rescale = false;
-      if (j == 0) {
-        m = m_new;
-      } else {
-        const bool need = m_new > m + 8.f;
-        rescale = __any_sync(0xffffffffu, need);
-        if (need) {
-          alpha = fast_exp2(m - m_new);
-          l *= alpha;
-          m = m_new;
+            for (int e = 0; e < 32; ++e) sv[cc * 32 + e] = keep >> e & 1 ? sv[cc * 32 + e] : -INFINITY;
+          }
         }
-      }
-      // A row that has seen no key yet has m = -inf: its scores are all -inf and p = 2^(-inf - 0) = 0.
-      const float m_use = m == -INFINITY ? 0.f : m;
-      const uint64_t a2 = f2_pack(a.scale_log2, a.scale_log2), b2 = f2_pack(-m_use, -m_use);
-      uint64_t lsum[4] = {0ull, 0ull, 0ull, 0ull};
-      if (whole) {
+        float t8[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t8[q] = fmax3(sv[q], sv[8 + q], sv[16 + q]);
+#pragma unroll
+        for (int e = 24; e < 56; e += 16)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) t8[q] = fmax3(t8[q], sv[e + q], sv[e + 8 + q]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t8[q] = fmaxf(t8[q], sv[56 + q]);
+        float mx = fmaxf(fmax3(t8[0], t8[1], t8[2]), fmax3(fmax3(t8[3], t8[4], t8[5]), t8[6], t8[7]));
+        *my_row = mx;
+        pair_sync(pair_bar);
+        mx = fmaxf(mx, *other_row) * a.scale_log2;
+        // The running maximum only moves when it grows by more than 2^8 (or from -inf). O and l are rescaled then, O by
+        // both threads of the row; it stands still: S is behind every P V before it.
+        const bool grow = mx > m + 8.f;
+        const bool rescale = __any_sync(0xffffffffu, grow);
+        const float alpha = !grow ? 1.f : m == -INFINITY ? 0.f : fast_exp2(m - mx);
+        if (grow) m = mx;
+        l *= alpha;
+        // A row that has seen no key yet has m = -inf and scores of -inf: p = 2^(-inf - 0) = 0.
+        const float m_use = m == -INFINITY ? 0.f : m;
+        const uint64_t a2 = f2_pack(a.scale_log2, a.scale_log2), b2 = f2_pack(-m_use, -m_use);
+        uint64_t lsum[2] = {0ull, 0ull};
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-          if (cc == 2 && !rescale) {  // keys 0..63 are in TMEM: let P V start on them (warp-uniform)
-            tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(&p_ready[wg][0]);
-          }
-          uint32_t pk[16];
+          uint32_t pk[8];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const int col = cc * 32 + e;
+          for (int e = 0; e < 16; e += 2) {
+            const int col = cc * 16 + e;
             float x0, x1, p0, p1;
             f2_unpack(f2_fma(f2_pack(sv[col], sv[col + 1]), a2, b2), x0, x1);
-            if (((e >> 1) & 3) == 3) {
-              exp2_poly2_nan(x0, x1, p0, p1);
-            } else {
-              p0 = fast_exp2(x0);
-              p1 = fast_exp2(x1);
-            }
-            lsum[(e >> 1) & 3] = f2_add(lsum[(e >> 1) & 3], f2_pack(p0, p1));
+            p0 = fast_exp2(x0);
+            p1 = fast_exp2(x1);
+            lsum[(e >> 1) & 1] = f2_add(lsum[(e >> 1) & 1], f2_pack(p0, p1));
             pk[e >> 1] = pack_16<F16>(p0, p1);
           }
-          tmem_st16(tS + cc * 16, pk);
+          tmem_st8(tS + cc * 8, pk);
         }
-      } else {
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const int col = cc * 32 + e;
-            float x0, x1;
-            f2_unpack(f2_fma(f2_pack(sv[col], sv[col + 1]), a2, b2), x0, x1);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            lsum[(e >> 1) & 3] = f2_add(lsum[(e >> 1) & 3], f2_pack(p0, p1));
-            pk[e >> 1] = pack_16<F16>(p0, p1);
-          }
-          tmem_st16(tS + cc * 16, pk);
-        }
-      }
-      float l0, l1, l2, l3;
-      f2_unpack(f2_add(lsum[0], lsum[1]), l0, l1);
-      f2_unpack(f2_add(lsum[2], lsum[3]), l2, l3);
-      l += (l0 + l1) + (l2 + l3);
-      if (rescale) {  // warp-uniform
+        if (rescale && left != n_tiles) {  // (the scores' registers are free now; before a window's first P V there is no O)
 #pragma unroll 1
-        for (int cc = 0; cc < D / 32; ++cc) {
-          uint32_t o[32];
-          tmem_ld32(tO + cc * 32, o);
-          tmem_ld_wait();
+          for (int cc = 0; cc < D / 64; ++cc) {
+            uint32_t o[32];
+            tmem_ld32(tO + cc * 32, o);
+            tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st32(tO + cc * 32, o);
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + cc * 32, o);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          pair_sync(pair_bar);  // either thread's arrival may start a P V into all of O
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        mbar_arrive_if(lane == 0, &p_ready[wg]);  // (one arrival per warp: 32 on one barrier take turns)
+        float l0, l1;
+        f2_unpack(f2_add(lsum[0], lsum[1]), l0, l1);
+        l += l0 + l1;
       }
-      tmem_st_wait();
-      tc_fence_before();
-      if (rescale || !whole) mbar_arrive(&p_ready[wg][0]);
-      mbar_arrive(&p_ready[wg][1]);
-    }
-    if (n_tiles > 0 && ok) ok = mbar_wait(&o_done[wg], 0, ab, 0x48 + wg);
-    if (ok && (wg == 0 || two)) {
-      tc_fence_after();
-      const long long row = (long long)(sq.q0 + tok);
-      const int head = head0 + r0 % ta.pack;
+      if (n_tiles > 0) {
+        mbar_wait_c(&o_done[wg], phases >> 1, ab, 0x48 + wg);
+        phases ^= 2;
+        tc_fence_after();
+      }
+      *my_row = l;  // for the row's sum over both halves (the last maxima have been read: O waited for both threads' P)
+      pair_sync(pair_bar);
+      l += *other_row;
+      pair_sync(pair_bar);  // (read before the next window's maxima)
+      const int tok = w.tok[wg] + r0 / ta.pack, head = w.head0 + r0 % ta.pack, split = w.split;
+      const bool mine = r0 < ta.pack * ta.tile_toks && tok < w.sq.nq && !abort_flag;
+      const long long row = (long long)w.sq.q0 + tok;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&win_empty[i & 1]);
       if (ta.n_split > 1) {
         // unnormalised fp32 row and its (m, l); a row without a key leaves only l = 0
-        const long long pr = ((long long)blockIdx.y * a.tq + row) * a.hq + head;
-        if (mine) *reinterpret_cast<float2*>(ta.part_ml + pr * 2) = make_float2(m, l);
-        float* dst = ta.part_o + pr * D;
+        const long long pr = ((long long)split * a.tq + row) * a.hq + head;
+        if (mine && half == 0) *reinterpret_cast<float2*>(ta.part_ml + pr * 2) = make_float2(m, l);
+        float* dst = ta.part_o + pr * D + half * (D / 2);
         if (n_tiles > 0) {
 #pragma unroll 1
-          for (int cc = 0; cc < D / 32; ++cc) {
+          for (int cc = 0; cc < D / 64; ++cc) {
             uint32_t r[32];
             tmem_ld32(tO + cc * 32, r);
             tmem_ld_wait();
@@ -421,25 +591,43 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
           }
         }
       } else {
-        const bool none = l == 0.f;  // no key seen: zeros (NaN sums stay NaN)
+        const bool none = l == 0.f;  // no key seen: zeros (a NaN stays)
         const float inv = 1.f / l;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + row * a.os_tok + head * a.os_head;
+        // 32 columns at a time through shared memory (16-byte pieces, the piece's place turned by the row), so that 4
+        // lanes store 64 contiguous bytes of a row: a row per thread would touch 32 lines with every store.
+        const unsigned long long at = reinterpret_cast<unsigned long long>(reinterpret_cast<uint16_t*>(a.out) +
+                                                                           row * a.os_tok + head * a.os_head + half * (D / 2));
+        const uint32_t some = none ? 0u : 0xffffffffu;
 #pragma unroll 1
-        for (int cc = 0; cc < D / 32; ++cc) {
-          uint32_t r[32];
-          if (n_tiles > 0) {
-            tmem_ld32(tO + cc * 32, r);
-            tmem_ld_wait();
-          }
-          uint32_t pk[16];
+        for (int cc = 0; cc < D / 64; ++cc) {
+#pragma unroll 1
+          for (int hh = 0; hh < 2; ++hh) {
+            uint32_t r[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            pk[e >> 1] = none ? 0u : pack_16<F16>(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv);
-          if (mine) {
+            for (int e = 0; e < 16; ++e) r[e] = 0;
+            if (n_tiles > 0) {
+              tmem_ld16(tO + cc * 32 + hh * 16, r);
+              tmem_ld_wait();
+            }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              reinterpret_cast<uint4*>(dst + cc * 32)[q] = make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+            for (int q = 0; q < 2; ++q) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                pk[e] = some & pack_16<F16>(__uint_as_float(r[8 * q + 2 * e]) * inv, __uint_as_float(r[8 * q + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 64 + (((hh * 2 + q) ^ ((lane >> 1) & 3)) << 4)) =
+                  make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
           }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int row_l = q * 8 + (lane >> 2);
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + row_l * 64 + (((lane & 3) ^ ((row_l >> 1) & 3)) << 4));
+            const unsigned long long to = __shfl_sync(0xffffffffu, at, row_l);
+            if (__shfl_sync(0xffffffffu, mine, row_l)) *reinterpret_cast<uint4*>(to + cc * 64 + (lane & 3) * 16) = v;
+          }
+          __syncwarp();
         }
       }
     }
@@ -447,7 +635,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 17) tmem_dealloc(tmem, 512);
 }
 
 // Joins the key ranges of split windows: out = sum_z 2^(m_z - M) O_z / sum_z 2^(m_z - M) l_z, M = max over the ranges
@@ -479,7 +667,7 @@ __global__ void __launch_bounds__(128) packed_merge_kernel(const __grid_constant
   for (int z = 0; z < ta.n_split; ++z) {
     const float2 ml = *reinterpret_cast<const float2*>(ta.part_ml + (z * step + wid) * 2);
     if (ml.y == 0.f) continue;  // no key of this range is visible: nothing was written
-    const float w = exp2f(ml.x - M);
+    const float w = ml.x == -INFINITY ? ml.y : exp2f(ml.x - M);  // (all scores NaN: so is the sum)
     L += w * ml.y;
     const float* o = ta.part_o + (z * step + wid) * D + lane * PER;
 #pragma unroll
@@ -619,7 +807,7 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   if (!aligned(cu_q, 4) || !aligned(cu_k, 4) || !aligned(k_lens, 4) || !aligned(out, 16) || out_tok % 8 || out_head % 8)
     return set_error(LBW_ERR_ALIGN, "%s: the output needs a 16-byte aligned pointer and strides", who);
   const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q, cu_q == cu_k && !k_lens);
-  if (p.windows >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
+  if (p.windows * 16 >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
   const long long need = (p.tile_floats + p.split_floats) * 4;
   if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
     return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who, need,
@@ -643,7 +831,7 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
     TileArgs ta = p.tile;
     ta.part_o = ws;
     ta.part_ml = ws ? ws + (long long)ta.n_split * tq * hq * head_dim : nullptr;
-    const dim3 grid((unsigned)p.windows, ta.n_split);
+    const dim3 grid((unsigned)(p.windows * ta.n_split));
     if (head_dim == 128)
       err = dtype == LBW_FP16 ? launch_tiles<128, true>(tmQ, tmK, tmV, a, ta, grid, st, s)
                               : launch_tiles<128, false>(tmQ, tmK, tmV, a, ta, grid, st, s);

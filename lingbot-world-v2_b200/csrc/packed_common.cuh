@@ -14,6 +14,25 @@ namespace lbw {
 LBW_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 LBW_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// mbar_wait with the waiting itself in one function for all sites: inlined, the loops and their error paths are a third
+// of the code of a kernel that has to stay in the instruction cache.
+static __device__ __noinline__ bool mbar_wait_long(uint32_t bar, uint32_t parity, int* status, volatile int* flag, int site) {
+  const long long t0 = clock64();
+  while (!mbar_test(bar, parity)) {
+    if (*flag) return false;
+    if (clock64() - t0 > LBW_WAIT_CYCLES) {
+      *flag = 1;
+      if (status) atomicCAS(status, 0, LBW_DEV_TIMEOUT | site);
+      return false;
+    }
+  }
+  return true;
+}
+LBW_DEV bool mbar_wait_c(uint64_t* bar, uint32_t parity, const Abort& ab, int site) {
+  const uint32_t a = smem_u32(bar);
+  return mbar_test(a, parity) || mbar_wait_long(a, parity, ab.status, ab.flag, site);
+}
+
 struct PackedArgs {
   const int* cu_q;    // [n_seqs + 1] first query row of each sequence
   const int* cu_k;    // [n_seqs + 1] first key row
@@ -48,32 +67,6 @@ LBW_DEV int packed_visible(const PackedArgs& a, const PackedSeq& s, int i) {
   if (!a.causal) return s.nk;
   const int n = i + 1 + s.nk - s.nq;
   return n < 0 ? 0 : (n < s.nk ? n : s.nk);
-}
-
-// Whole warp: the sequence b and its local item l of global item w, where sequence b has count(b) items; false when w
-// lies past the last one. Each lane counts one sequence, 32 of them per step.
-template <typename F>
-LBW_DEV bool packed_find(int n_seqs, long long w, F count, int& b, long long& l) {
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int b0 = 0; b0 < n_seqs; b0 += 32) {
-    const long long own = b0 + lane < n_seqs ? (long long)count(b0 + lane) : 0;
-    long long upto = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > w);
-    if (hit) {
-      const int at = __ffs(hit) - 1;
-      b = b0 + at;
-      l = w - before - __shfl_sync(0xffffffffu, upto - own, at);
-      return true;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return false;
 }
 
 // The whole block of NT threads: an item of a list in which sequence b has n.x items (SEARCH_Y: n.y) of (n.x, n.y) =

@@ -258,6 +258,12 @@ def test_packed_attention_peaked_and_huge_scores(cuda_dev):
 def test_packed_attention_nan_stays_with_its_sequence(cuda_dev):
     """A NaN key or value reaches every row that sees it and no other sequence; NaN keys ahead of a row do not."""
     import lbw_b200.kernels as K
+    for at in range(0, 128, 5):                                             # every place of a whole key tile
+        q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, [300, 20], [300, 300], 4, 2, 64, BF)
+        clean = K.packed_attention(q, k, v, cu_q, cu_k)
+        k[128 + at], k[300 + at] = float("nan"), float("nan")
+        out = K.packed_attention(q, k, v, cu_q, cu_k)
+        assert torch.equal(out[:128 + at], clean[:128 + at]) and torch.isnan(out[128 + at:].float()).all()
     for lens in ([130, 200, 60], [1, 1, 1]):
         ks = [130, 200, 60]
         q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, lens, ks, 4, 2, 128, BF)
