@@ -711,7 +711,8 @@ static int launch_tiles(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
 // Query heads side by side in a tile: the divisor d of the group that needs the fewest 128-row tiles for sequences of
 // `avg` tokens, ceil(avg / floor(128 / d)) tiles for each of hq / d head tiles; the larger divisor where two are equal.
 // (Group 4: always 4. Group 6: 6 below 21 tokens, where one tile takes all heads, 2 for long sequences, which it fills
-// to 128 of 128 rows; 6 heads fill 126.)
+// to 128 of 128 rows; 6 heads fill 126.) Measured (us, this rule / always one head, 32 heads over 8, 128 wide, causal):
+// 256 x 20 tokens 63 / 214, 128 x 50 44 / 115, 32 x 300 69 / 102, 8 x 1,000 89 / 96, 2 x 4,000 264 / 281.
 static int pick_pack(int group, long long avg) {
   int best = 1;
   double best_cost = 1e300;
@@ -727,7 +728,10 @@ static int pick_pack(int group, long long avg) {
   return best;
 }
 
-// Rows per kv head (queries x group) up to which a sequence is packed_split_kernel's, which has 16 in a unit.
+// Rows per kv head (queries x group) up to which a sequence is packed_split_kernel's, which has 16 in a unit: it reads the
+// keys and values once for each unit, the tile kernel once for 256 rows. Measured (us, split / tile kernel, 8 kv heads,
+// 128 wide) at 1, 16 and 32 rows: 32 x 16,384 keys 329 / 417, 340 / 425, 655 / 425; 8 x 4,096 33 / 40, 35 / 37, 45 / 37;
+// 1 x 30,000 30 / 40, 34 / 40, 50 / 41; 1 x 1,000 9 / 14, 10 / 14, 12 / 15; 128 x 500 54 / 65, 70 / 67, 133 / 66.
 constexpr int SHORT_ROWS = 16;
 
 // The call's launch plan, from the host's numbers alone. The sequences' own lengths are on the device: where they may be
@@ -758,6 +762,11 @@ static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, i
   if (pairs > tq) pairs = tq;
   p.windows = pairs * p.tile.head_tiles;
   const long long key_tiles = (tk + 127) / 128;
+  // Few windows: their keys are cut into ranges while the windows fill the SMs at most once, each range of 4 key tiles or
+  // more, 16 ranges at most (a row's partial results are merged one after the other). Measured (us, with / without, 8
+  // heads): 200 queries of 30,000 keys 53 / 417, of 8,192 32 / 120, of 1,000 20 / 23; 1,000 of 8,192 50 / 121; 500 of 500
+  // 15 / 15. Ranges of 2 tiles: 17 at 200 of 1,000, but 18 at 500 of 500; up to 64 ranges: 35 for 28 at 64 of 8,192; as
+  // many as fill the SMs twice: 62 for 50 at 1,000 of 8,192.
   long long split = p.windows > 0 ? num_sms() / p.windows : 1;
   if (split > key_tiles / 4) split = key_tiles / 4;
   if (split > 16) split = 16;

@@ -11,6 +11,11 @@
 //                maximum, sums and 16 x D accumulator (mma.sync m16n8k16), joined over the 8 warps at the unit's end
 // mma.sync and not tcgen05: the rows of a unit fill an eighth of a 128-row tile, and 16 rows are enough to read at full
 // rate (a warp spends ~150 instructions on 16 keys = 8 KB; the SM's share of the memory rate is 23 bytes a clock).
+// Bound: the bytes of K and V. Measured (B200, bf16, 128-wide heads, 8 kv heads, both kernels, replayed from a graph):
+// 32 sequences of 16,384 keys 329 us with 1 row per kv head, 340 with 16 (6.5 and 6.3 TB/s: a plain copy's rate);
+// 128 x 500 keys 53 and 70 us (5.0 and 3.7 TB/s: a unit's join of its warps is not hidden behind 8 tiles of loads);
+// 1 x 30,000 keys 30 and 34 us (4.1 and 3.7 TB/s); 1 x 1,000 keys 8.5 and 10 us, which is two launches, the look-up of
+// the sequences and one trip to memory.
 #include "host_common.cuh"
 #include "packed_common.cuh"
 #include "packed_host.cuh"
@@ -60,10 +65,11 @@ LBW_DEV longlong2 split_count(const PackedArgs& a, long long max_rows, int b) {
   return make_longlong2(units, units * ((s.nk + ps::KEYS - 1) / ps::KEYS));
 }
 
-// Key tiles of each CTA: an equal share, but no less than two (below that the parts cost more than they bring).
+// Key tiles of each CTA: an equal share. (A minimum of 2 or 4 measures the same or slower: 1 x 1,000 keys 8.8 / 9.5 us
+// against 8.5, 4 x 500 keys of 2 kv heads 8.7 / 9.3 against 8.2.)
 LBW_DEV long long split_share(long long total, int ctas) {
   const long long w = (total + ctas - 1) / ctas;
-  return w < 2 ? 2 : w;
+  return w < 1 ? 1 : w;
 }
 
 // Where a CTA stands in the list: a unit of sequence b, from its key tile t0 on.
@@ -330,13 +336,18 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
   pdl_wait();
 }
 
-// Joins the units that crossed CTAs and writes the rows of sequences without keys. One block per unit.
+// Joins the units that crossed CTAs and writes the rows of sequences without keys. Block (unit, y) has the y-th share of
+// the unit's rows, a warp per row, or two or four warps where the share is fewer rows than warps (`W`: they take the
+// row's parts in turn), with the loads of 8 parts in flight. Many blocks for few units: one sequence of 8 kv heads over
+// 148 CTAs leaves 19 parts a row, and one block per unit reading 16 rows of them one by one took 20 us of 55.
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant__ PackedArgs a, long long max_rows,
                                                           int ctas, const float* __restrict__ part_o,
                                                           const float* __restrict__ part_ml) {
+  constexpr int PER = D / 32, UN = 8;
   __shared__ longlong2 tmp[5];
   __shared__ PackedAt at_s;
+  __shared__ float s_acc[4][D], s_l[4];
   const PackedAt at = packed_locate<128, false>(
       a, [&](int b) { return split_count(a, max_rows, b); }, [&](longlong2) { return (long long)blockIdx.x; }, tmp,
       &at_s);
@@ -347,25 +358,64 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
   const long long share = split_share(at.total_y, ctas);
   const long long t_first = at.before_y + at.local * n_tiles;
   const int c0 = (int)min(t_first / share, ctas - 1ll);
-  const int c1 = n_tiles ? (int)min((t_first + n_tiles - 1) / share, ctas - 1ll) : c0;
-  if (n_tiles > 0 && c0 == c1) return;
+  const int c1 = n_tiles ? (int)min((t_first + n_tiles - 1) / share, ctas - 1ll) : c0 - 1;
+  if (c0 == c1) return;
   const int head = (int)(at.local % a.hk), row0 = (int)(at.local / a.hk) * ps::ROWS;
   const int rows = min(sq.nq * a.group - row0, ps::ROWS);
-  const int lane = threadIdx.x & 31;
-  constexpr int PER = D / 32;
-  for (int r = threadIdx.x >> 5; r < rows; r += 4) {
-    float M = -INFINITY, L = 0.f, acc[PER] = {};
-    if (n_tiles > 0) {
-      for (int c = c0; c <= c1; ++c) M = fmaxf(M, part_ml[((2ll * c + (c == c0)) * ps::ROWS + r) * 2]);
-      for (int c = c0; c <= c1; ++c) {
-        const long long at_row = (2ll * c + (c == c0)) * ps::ROWS + r;
-        const float2 ml = *reinterpret_cast<const float2*>(part_ml + at_row * 2);
-        const float k = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-        L += k * ml.y;
+  const int rows_y = (rows + gridDim.y - 1) / gridDim.y;
+  const int r0 = blockIdx.y * rows_y, r1 = min(rows, r0 + rows_y);
+  const int W = rows_y >= 4 ? 1 : rows_y >= 2 ? 2 : 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int rb = r0; rb < r1; rb += 4 / W) {
+    const int r = rb + warp / W, part = warp % W;
+    float L = 0.f, acc[PER] = {};
+    if (r < r1) {
+      float M = -INFINITY;
+      for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, part_ml[((2ll * c + (c == c0)) * ps::ROWS + r) * 2]);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] += k * part_o[at_row * D + lane * PER + e];
+      for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+      for (int cb = c0 + part; cb <= c1; cb += W * UN) {
+        float2 ml[UN];
+        float f[UN][PER];
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+          const int c = cb + i * W;
+          ml[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+          for (int e = 0; e < PER; ++e) f[i][e] = 0.f;
+          if (c > c1) continue;
+          const long long at_row = (2ll * c + (c == c0)) * ps::ROWS + r;
+          ml[i] = *reinterpret_cast<const float2*>(part_ml + at_row * 2);
+#pragma unroll
+          for (int e = 0; e < PER; e += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(part_o + at_row * D + lane * PER + e);
+            f[i][e] = v.x;
+            f[i][e + 1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < UN; ++i) {
+          const float k = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
+          L += k * ml[i].y;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] += k * f[i][e];
+        }
       }
     }
+    if (W > 1) {  // (the same for the whole block)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) s_acc[warp][lane * PER + e] = acc[e];
+      if (lane == 0) s_l[warp] = L;
+      __syncthreads();
+      if (part == 0)
+        for (int w = warp + 1; w < warp + W; ++w) {
+          L += s_l[w];
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] += s_acc[w][lane * PER + e];
+        }
+      __syncthreads();
+    }
+    if (part > 0 || r >= r1) continue;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int tok = (row0 + r) / a.group, hh = head * a.group + (row0 + r) % a.group;
     uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) +
@@ -391,6 +441,11 @@ static int launch_split_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const 
     if (err) return err;
     attr[dix] = true;
   }
+  // Row tiles: one per sequence of at most 16 rows; else at most one per sequence beyond tq * group / 16 full ones.
+  const long long per_tok = (a.group + ps::ROWS - 1) / ps::ROWS;
+  long long units = max_rows <= ps::ROWS ? a.n_seqs : (long long)a.tq * a.group / ps::ROWS + a.n_seqs;
+  if (units > a.tq * per_tok) units = a.tq * per_tok;
+  if (units * a.hk >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "packed_attention: %lld units", units * a.hk);
   const int ctas = num_sms();
   float* part_ml = ws + 2ll * ctas * ps::ROWS * D;
   const uint16_t* q16 = reinterpret_cast<const uint16_t*>(q);
@@ -403,12 +458,14 @@ static int launch_split_t(const CUtensorMap& tmK, const CUtensorMap& tmV, const 
     err = cuda_check(cudaGetLastError(), "packed_attention split launch");
   }
   if (err) return err;
-  // Row tiles: one per sequence of at most 16 rows; else at most one per sequence beyond tq * group / 16 full ones.
-  const long long per_tok = (a.group + ps::ROWS - 1) / ps::ROWS;
-  long long units = max_rows <= ps::ROWS ? a.n_seqs : (long long)a.tq * a.group / ps::ROWS + a.n_seqs;
-  if (units > a.tq * per_tok) units = a.tq * per_tok;
-  return launch_dependent("packed_attention join launch", packed_join_kernel<D, F16>, dim3((unsigned)(units * a.hk)), 128,
-                          0, s, a, max_rows, ctas, ws, part_ml);
+  // A block per row of the unit (of the batch's mean) while that makes less than four blocks per SM.
+  const long long mean = ((long long)a.tq * a.group + a.n_seqs - 1) / a.n_seqs;
+  long long row_blocks = 4ll * ctas / (units * a.hk);
+  if (row_blocks > mean) row_blocks = mean;
+  if (row_blocks > ps::ROWS) row_blocks = ps::ROWS;
+  const dim3 grid((unsigned)(units * a.hk), row_blocks < 1 ? 1u : (unsigned)row_blocks);
+  return launch_dependent("packed_attention join launch", packed_join_kernel<D, F16>, grid, 128, 0, s, a, max_rows, ctas,
+                          ws, part_ml);
 }
 
 int launch_split(const void* k, long long k_tok, long long k_head, const void* v, long long v_tok, long long v_head,

@@ -4,7 +4,6 @@ Every wrapper validates dtypes/devices, passes raw pointers and the current CUDA
 non-zero status into ValueError / LbwError. Outputs may be passed in (written in place) or are
 allocated here.
 """
-import contextlib
 import ctypes
 import functools
 import math
@@ -747,39 +746,47 @@ def _device_index(who, *tensors):
     """Index of the CUDA device that holds all the given tensors (None skipped); these operators have no gradient."""
     dev = tensors[0].get_device()
     grad = torch.is_grad_enabled()
+    if dev < 0:
+        require_cuda(*tensors)
     for t in tensors:
         if t is not None:
-            if dev < 0 or t.get_device() < 0:
-                require_cuda(*tensors)
             if t.get_device() != dev:
+                require_cuda(*tensors)
                 raise ValueError(f"{who}: tensors on different devices")
             if grad and t.requires_grad:
                 raise ValueError(f"{who} has no gradient: call it under torch.no_grad() or with detached tensors")
     return dev
 
 
-def _on(dev):
-    """Context in which device `dev` is the current one (the library launches on the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+def _launch(dev, fn, *args):
+    """fn(*args, the current stream of device dev) with dev as the current device (the library launches there)."""
+    if torch.cuda.current_device() == dev:
+        return fn(*args, raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, raw_stream(dev))
 
 
 def _rows3(who, name, t, dtype=None, dim=None, written=False):
     """(tokens, heads, head_dim, token stride, head stride) of a [tokens, heads, head_dim] or [1, tokens, heads,
     head_dim] tensor with a contiguous head_dim."""
     shape, stride = t.shape, t.stride()
-    if len(shape) == 4 and shape[0] == 1:
+    if len(shape) != 3:
+        if len(shape) != 4 or shape[0] != 1:
+            raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(shape)}")
         shape, stride = shape[1:], stride[1:]
-    if len(shape) != 3 or shape[1] < 1:
+    tokens, heads, d = shape
+    tok, head, inner = stride
+    if heads < 1:
         raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
-    if dim is not None and shape[2] != dim:
-        raise ValueError(f"{who}: head_dim of {name} is {shape[2]}, expected {dim}")
-    if stride[2] != 1 and shape[2] > 1:
+    if dim is not None and d != dim:
+        raise ValueError(f"{who}: head_dim of {name} is {d}, expected {dim}")
+    if inner != 1 and d > 1:
         raise ValueError(f"{who}: {name} needs a contiguous head_dim")
-    if written and ((stride[0] == 0 and shape[0] > 1) or (stride[1] == 0 and shape[1] > 1)):
+    if written and ((tok == 0 and tokens > 1) or (head == 0 and heads > 1)):
         raise ValueError(f"{who}: {name} is an expanded tensor")
-    return (*shape, stride[0], stride[1])
+    return tokens, heads, d, tok, head
 
 
 def _positions(who, positions, tokens, rope):
@@ -823,10 +830,8 @@ def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
     if o_tokens != tokens or o_heads != heads:
         raise ValueError(f"{who}: out is {tuple(out.shape)}, x {tuple(x.shape)}")
     pos = _positions(who, positions, tokens, rope)
-    with _on(dev):
-        check(load().lbw_axial_rope(x.data_ptr(), x_tok, x_head, out.data_ptr(), o_tok, o_head, tokens, heads, dim,
-                                    DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0, raw_stream(dev)), who,
-              launches=1 if tokens else 0)
+    check(_launch(dev, load().lbw_axial_rope, x.data_ptr(), x_tok, x_head, out.data_ptr(), o_tok, o_head, tokens, heads,
+                  dim, DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0), who, launches=1 if tokens else 0)
     return out
 
 
@@ -892,11 +897,15 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
             raise ValueError(f"{who}: v {tuple(v.shape)} / v_out {tuple(v_out.shape)} do not match q and k_out")
         seg_v = HEAD_ROWS.pack(v.data_ptr(), v_out.data_ptr(), 0, v_tok, v_head, vo_row, vo_head, hv, 0)
     pos = (None, 32, 0, 0) if rope is None else _positions(who, positions, tokens, rope)
-    with _on(dev):
-        check(load().lbw_qk_headnorm_rope(seg_q, seg_k, seg_v, tokens, dim, DTYPES[dtype], eps, *pos,
-                                          None if rope is None else rope.ref, rows, rows_bits, ko_rows,
-                                          raw_stream(dev)), who, launches=1 if tokens else 0)
+    check(_launch(dev, load().lbw_qk_headnorm_rope, seg_q, seg_k, seg_v, tokens, dim, DTYPES[dtype], eps, *pos,
+                  None if rope is None else rope.ref, rows, rows_bits, ko_rows), who, launches=1 if tokens else 0)
     return q_out, k_out
+
+
+def _int32(who, name, t, n):
+    """Check that t is a contiguous int32 vector of n values."""
+    if n < 0 or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{who}: {name} must be contiguous int32 [{max(n, 0)}], got {tuple(t.shape)} {t.dtype}")
 
 
 @functools.lru_cache(4096)
@@ -946,9 +955,11 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
     if v_rows != tk or hv != hk:
         raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
     n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
-    for name, t, want in (("cu_q", cu_q, n + 1), ("cu_k", cu_k, n + 1), ("k_lens", k_lens, n)):
-        if t is not None and (n < 0 or t.dtype != torch.int32 or t.shape != (want,) or not t.is_contiguous()):
-            raise ValueError(f"{who}: {name} must be contiguous int32 [{max(want, 0)}], got {tuple(t.shape)} {t.dtype}")
+    _int32(who, "cu_q", cu_q, n + 1)
+    if cu_k is not cu_q:
+        _int32(who, "cu_k", cu_k, n + 1)
+    if k_lens is not None:
+        _int32(who, "k_lens", k_lens, n)
     if max_q is None:
         max_q = 0
     elif max_q < 0:
@@ -967,10 +978,9 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
         ws_bytes = workspace.numel() * workspace.element_size()
     elif ws_bytes:
         workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
-    with _on(dev):
-        check(load().lbw_packed_attention(
-            q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head, out.data_ptr(),
-            o_tok, o_head, pq, pk, None if k_lens is None else k_lens.data_ptr(), n, tq, tk, hq, hk, dim, DTYPES[dtype],
-            1 if causal else 0, scale, max_q, None if workspace is None else workspace.data_ptr(), ws_bytes,
-            raw_stream(dev)), who, launches=launches)
+    check(_launch(dev, load().lbw_packed_attention, q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head,
+                  v.data_ptr(), v_tok, v_head, out.data_ptr(), o_tok, o_head, pq, pk,
+                  None if k_lens is None else k_lens.data_ptr(), n, tq, tk, hq, hk, dim, DTYPES[dtype],
+                  1 if causal else 0, scale, max_q, None if workspace is None else workspace.data_ptr(), ws_bytes), who,
+          launches=launches)
     return out
