@@ -267,7 +267,9 @@ typedef struct {
 /* Every head vector of q and k: x * rsqrt(mean(x^2) + eps) * gamma, then the rotation (rope NULL: none), fp32 with one
  * rounding. With k_rows (int32 or int64 [tokens], k_rows_bits) token t's k goes to row k_rows[t] of k->out, and v, if
  * given, is copied to row k_rows[t] of v->out (a cache of out_rows rows); a row outside [0, out_rows) is not written.
- * Without k_rows the rows are the tokens. Two tokens with the same row: either is kept, head by head. */
+ * Without k_rows the rows are the tokens. Two tokens with the same row leave a mix of both
+ * there. The sums of squares are fp32: values beyond 1e18 make them infinite and the head zero. out may be x (k and v:
+ * without k_rows), with the same strides. */
 int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
                          int head_dim, int dtype, float eps, const void* positions, int pos_bits, long long pos_tok,
                          long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
@@ -286,7 +288,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
  * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
  * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels
- * that such a call enqueues). */
+ * that such a call enqueues). out may be q, with the same strides. */
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
                                    int same_lens, long long* bytes, int* launches);
 int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const void* k, long long k_tok,

@@ -294,6 +294,13 @@ static int check_seg(const char* who, const char* name, const void* x, const voi
   return LBW_OK;
 }
 
+// In place every vector has to stay where it is: others read it. moved: rows go elsewhere.
+static int check_in_place(const char* who, const HeadSeg& g, long long tokens, bool moved) {
+  if (g.x == g.out && (moved || (tokens > 1 && g.xs_tok != g.os_tok) || (g.heads > 1 && g.xs_head != g.os_head)))
+    return set_error(LBW_ERR_INVALID, "%s: in place with other strides or rows", who);
+  return LBW_OK;
+}
+
 static int check_common(const char* who, long long tokens, int head_dim, int dtype, const void* positions,
                         int pos_bits, const lbw_rope_axes* rope) {
   if (dtype != LBW_BF16 && dtype != LBW_FP16 && dtype != LBW_FP32)
@@ -380,6 +387,7 @@ int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, 
     return err;
   HeadArgs a{};
   a.seg[0] = HeadSeg{x, out, nullptr, x_tok, x_head, out_tok, out_head, heads, 0};
+  if ((err = check_in_place(who, a.seg[0], tokens, false))) return err;
   a.tokens = tokens;
   a.dim = head_dim;
   a.pos = positions;
@@ -418,6 +426,8 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
       return set_error(LBW_ERR_ALIGN, "%s: gamma of %s is misaligned", who, names[i]);
     a.seg[i] = HeadSeg{r.x, r.out, r.gamma, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads, r.gamma_f32};
   }
+  for (int i = 0; i < 3; ++i)
+    if (in[i] && (err = check_in_place(who, a.seg[i], tokens, i > 0 && k_rows))) return err;
   a.tokens = tokens;
   a.dim = head_dim;
   a.eps = eps;

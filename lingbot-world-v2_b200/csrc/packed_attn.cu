@@ -809,7 +809,8 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   int err = check_packed(tq, tk, hq, hk, head_dim, n_seqs);
   if (err) return err;
   if (dtype != LBW_BF16 && dtype != LBW_FP16) return set_error(LBW_ERR_INVALID, "%s: dtype %d (bf16 or fp16)", who, dtype);
-  if (!(softmax_scale > 0.f) || isinf(softmax_scale))
+  const float scale_log2 = softmax_scale * 1.4426950408889634f;  // (log2 e: the exponentials are powers of two)
+  if (!(scale_log2 > 0.f) || isinf(scale_log2))
     return set_error(LBW_ERR_INVALID, "%s: softmax_scale %g (a positive number)", who, (double)softmax_scale);
   if (tq == 0 || n_seqs == 0) return LBW_OK;
   if (!q || !out || !cu_q || !cu_k || (tk > 0 && (!k || !v))) return set_error(LBW_ERR_INVALID, "%s: null pointer", who);
@@ -821,10 +822,13 @@ int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const
   if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
     return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who, need,
                      ws_bytes);
+  if (tk > 0 && (out == k || out == v)) return set_error(LBW_ERR_INVALID, "%s: out is k or v", who);
+  if (out == q && ((tq > 1 && q_tok != out_tok) || (hq > 1 && q_head != out_head)))
+    return set_error(LBW_ERR_INVALID, "%s: out is q with other strides", who);
   int* st = device_status(&err);
   if (!st) return err;
   const PackedArgs a{cu_q, cu_k, k_lens, n_seqs, (int)tq, (int)tk, hq, hk, hq / hk, causal != 0,
-                     softmax_scale * 1.4426950408889634f, out, out_tok, out_head};
+                     scale_log2, out, out_tok, out_head};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   float* ws = reinterpret_cast<float*>(workspace);
   if (p.tiles) {

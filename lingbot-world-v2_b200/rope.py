@@ -132,3 +132,6 @@ class AxialRope:
             self.c.axis[i] = self.axis_of_pair[i]
             self.c.step[i] = round(f / (2 * math.pi) * 2.0 ** 64) % (1 << 64)
         self.ref = ctypes.byref(self.c)
+
+    def __reduce__(self):
+        return AxialRope, (self.sections, self.theta, self.layout, self.spectrum, self.scale)

@@ -316,6 +316,40 @@ def test_packed_attention_offsets_past_32_bits(cuda_dev):
         assert po.within(out[:n], want[:n], bound[:n]) <= 1
 
 
+def test_packed_attention_over_many_short_sequences(cuda_dev):
+    """3,000 sequences, most of them empty or of one token, in both kernels' hands; the output in the query's place."""
+    import lbw_b200.kernels as K
+    gen = torch.Generator().manual_seed(3)
+    q_lens = (torch.randint(0, 3, (3000,), generator=gen) * torch.randint(0, 2, (3000,), generator=gen)).tolist()
+    k_lens = [n + int(i % 7 == 0) * (i % 40) for i, n in enumerate(q_lens)]
+    q_lens[1500], k_lens[1500], q_lens[2999], k_lens[2999] = 70, 150, 9, 9
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, 4, 2, 64, BF)
+    want, bound = po.attention(q, k, v, cu_q, cu_k)
+    assert po.within(K.packed_attention(q, k, v, cu_q, cu_k), want, bound) <= 1
+    for lens in (None, 70):
+        x = q.clone()
+        assert K.packed_attention(x, k, v, cu_q, cu_k, out=x, max_q=lens) is x
+        assert po.within(x, want, bound) <= 1
+
+
+@pytest.mark.parametrize("heads,q_lens,k_lens", [((4, 4), [200], [3000]), ((8, 1), [2], [9000]), ((8, 2), [1] * 3, [5000, 64, 1])])
+def test_packed_attention_in_place_where_keys_are_split(cuda_dev, heads, q_lens, k_lens):
+    """Blocks that share a query's keys all read it before any of them writes its row."""
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, *heads, 128, BF)
+    want = K.packed_attention(q, k, v, cu_q, cu_k)
+    for _ in range(5):
+        x = q.clone()
+        assert torch.equal(K.packed_attention(x, k, v, cu_q, cu_k, out=x), want)
+
+
+def test_packed_attention_takes_a_batch_dimension_of_one(cuda_dev):
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, [30, 1], [30, 50], 4, 2, 64, BF)
+    out = K.packed_attention(q[None], k[None], v[None], cu_q, cu_k)
+    assert out.shape == (1, 31, 4, 64) and torch.equal(out[0], K.packed_attention(q, k, v, cu_q, cu_k))
+
+
 def test_packed_attention_refuses(cuda_dev):
     import lbw_b200.kernels as K
     x = torch.zeros(4, 2, 64, dtype=BF, device=cuda_dev)
@@ -419,6 +453,40 @@ def test_captured_step_follows_new_lengths_and_rows(cuda_dev):
         assert torch.equal(kc, before)
         want, bound = po.attention(q16, kc, vc, cu_q, cu_k, k_lens)
         assert po.within(out, want, bound) <= 1
+
+
+@pytest.mark.parametrize("tq,max_q", [(200, None), (2000, None), (2000, 700)])
+def test_captured_prompts_follow_new_lengths(cuda_dev, tq, max_q):
+    """Graphs of the tile kernel with the keys in ranges (tq 200) and without, next to the kernel for single tokens; two
+    graphs with a workspace each, replayed side by side."""
+    import lbw_b200.kernels as K
+    hq, hk, d, tk, n = 8, 2, 128, 6000, 3
+    q, k, v = _randn(cuda_dev, 1, tq, hq, d), _randn(cuda_dev, 2, tk, hk, d), _randn(cuda_dev, 3, tk, hk, d)
+    sets = []
+    for _ in range(2):
+        cu_q, cu_k = (torch.zeros(n + 1, dtype=torch.int32, device=cuda_dev) for _ in range(2))
+        ws = K.packed_attention_workspace(tq, tk, hq, hk, d, n, cuda_dev, max_q=max_q)
+        out, side, graph = torch.empty_like(q), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side):
+            K.packed_attention(q, k, v, cu_q, cu_k, out=out, max_q=max_q, workspace=ws)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            K.packed_attention(q, k, v, cu_q, cu_k, out=out, max_q=max_q, workspace=ws)
+        sets.append((cu_q, cu_k, out, side, graph, ws))
+    for lens in (([150, 1, 2], [150, 3000, 2]), ([1, 130, 60], [2500, 1300, 2000]), ([0, 3, 197], [0, 5000, 200])):
+        want, bound = po.attention(q, k, v, _cu(lens[0], cuda_dev), _cu(lens[1], cuda_dev))
+        for cu_q, cu_k, out, *_ in sets:
+            cu_q.copy_(_cu(lens[0], cuda_dev))
+            cu_k.copy_(_cu(lens[1], cuda_dev))
+            out.zero_()
+        torch.cuda.synchronize()
+        for _, _, _, side, graph, _ in sets:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        rows = sum(lens[0])
+        for _, _, out, *_ in sets:
+            assert po.within(out[:rows], want[:rows], bound[:rows]) <= 1 and bool((out[rows:] == 0).all())
 
 
 def test_two_streams_at_once(cuda_dev):

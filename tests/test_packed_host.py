@@ -1,6 +1,8 @@
 """Packed-sequence operators without a GPU: the rotation's description, refusals, and the C entries' argument checks."""
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -127,3 +129,33 @@ def test_packed_attention_refuses_a_small_workspace(lib):
     assert rc == L.LBW_ERR_INVALID and "workspace" in L.last_error()
     assert lib.lbw_packed_attention_workspace(1, 100, 8, 3, 128, 1, 1, 0, ctypes.byref(n), None) == L.LBW_ERR_SHAPE
     assert lib.lbw_packed_attention_workspace(1, 100, 8, 2, 128, 1, 1, 0, None, None) == L.LBW_ERR_INVALID
+
+
+def test_in_place_calls_that_would_race_are_refused(lib):
+    """x as its own output with other strides or rows, keys or values as the output of the attention."""
+    axial = dict(x=P, x_tok=1024, x_head=64, out=P, out_tok=2048, out_head=64, tokens=5, heads=2, dim=64, dtype=0, pos=P,
+                 bits=32, pos_tok=1, pos_axis=1, rope=_rope(), inverse=0)
+    assert lib.lbw_axial_rope(*axial.values(), None) == L.LBW_ERR_INVALID and "in place" in L.last_error()
+    there = _rows(out=8192)
+    for q, k, v, rows in ((_rows(out_head=128), there, None, None), (there, _rows(), None, P), (there, there, _rows(), P)):
+        assert lib.lbw_qk_headnorm_rope(q, k, v, 5, 64, 0, 1e-6, P, 32, 1, 1, _rope(), rows, 64, 9, None) == L.LBW_ERR_INVALID
+        assert "in place" in L.last_error()
+    far = ctypes.c_void_p(1 << 20)
+    for q, k, v, out_tok in ((far, P, far, 1024), (far, far, P, 1024), (P, far, far, 2048)):
+        assert lib.lbw_packed_attention(q, 1024, 64, k, 1024, 64, v, 1024, 64, P, out_tok, 64, P, P, None, 2, 100, 100, 8, 2,
+                                        64, 0, 1, 0.1, 0, P, 1 << 40, None) == L.LBW_ERR_INVALID
+        assert "out is" in L.last_error()
+
+
+def test_packed_attention_refuses_a_scale_out_of_range(lib):
+    for scale in (3e38, 1e-46):                                             # times log2 e: infinite, zero
+        assert lib.lbw_packed_attention(P, 1024, 64, P, 1024, 64, P, 1024, 64, P, 1024, 64, P, P, None, 2, 100, 100, 8, 2,
+                                        64, 0, 1, scale, 0, P, 1 << 40, None) == L.LBW_ERR_INVALID
+        assert "softmax_scale" in L.last_error()
+
+
+def test_axial_rope_can_be_copied_and_pickled():
+    """A model that holds one is deep-copied and saved whole."""
+    r = rope.AxialRope((8, 4, 4), theta=500.0, layout="half", spectrum="head", scale=(1.0, 0.5, 2.0))
+    for c in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert bytes(c.c) == bytes(r.c) and c.scale == r.scale and c.axis_of_pair == r.axis_of_pair
