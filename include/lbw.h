@@ -283,8 +283,8 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
  * int32, read when the kernels run (a captured graph may be replayed with others); starts and lengths that do not fit
  * the tensors are cut to what does.
  * q, out: [tq, hq, head_dim]; k, v: [tk, hk, head_dim]; hq a multiple of hk, query head h uses kv head h / (hq / hk);
- * head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A non-finite value in a visible key or value reaches the
- * rows that see it; in a value row it also reaches rows of the same sequence that stand before it by less than 128 keys.
+ * head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A value that is not finite makes its column infinite or NaN
+ * in the rows that see it, a NaN key all of such a row; no other row is touched.
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
  * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
  * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels

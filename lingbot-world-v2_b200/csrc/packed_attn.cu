@@ -17,7 +17,9 @@
 //                    so that the next Q, K and S are under way before the last rows of the present window are written
 //   warp 18          watches the K/V ring for the issuer (its arrival folds "V(j) and K(j + 1) landed" into the barrier that
 //                    announces the primary's P) and clears the value rows past the sequence's last key: they belong to
-//                    another sequence or to nobody, and 0 * NaN would reach the sum
+//                    another sequence or to nobody, and 0 * NaN would reach the sum. On the diagonal it looks for values
+//                    that are not finite, which rows may not see: they are taken out of the tile and noted, and the
+//                    epilogue adds them to the rows that do see them
 // P is written over S in TMEM, so a tile's chain is softmax, P V, next S; the two tiles take turns at the tensor pipe. The
 // running maximum moves only when it grows by more than 2^8.
 // What it measured (B200, D = 128, non-causal, cycles of one step = both tiles against 128 keys, 2,048 of them MMA at
@@ -136,6 +138,96 @@ LBW_DEV bool pair_all(int id, bool ok) {
   return r != 0;
 }
 
+// What a window keeps of the values that are not finite: for each column the first key with a NaN, with +inf and with
+// -inf, 10 bits each, counted from `base` (the diagonal spans less than 640 keys); all ones: none.
+constexpr uint32_t NO_KEY = 0x3ff, ALL_FINITE = 0x3fffffff;
+
+// Whether rows [lo, hi) of a value tile (128 rows x D, swizzled) hold an infinity or a NaN: one answer for the warp. This
+// look costs 2 to 7% of the time of short causal sequences (64 x 300..900 tokens 361 -> 375 us, 256 x 64..300 146 -> 156)
+// and nothing that can be measured beyond 10,000 tokens or without a mask; unrolled by 4 or 1, or not inlined: 1% more.
+template <int D, bool F16>
+LBW_DEV bool v_not_finite(const uint8_t* tile, int lo, int hi) {
+  uint32_t top = 0;
+  auto take = [&](uint32_t x) {  // larger magnitude of either half, NaN above all
+    if constexpr (F16) {
+      const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&top), __habs2(*reinterpret_cast<__half2*>(&x)));
+      top = *reinterpret_cast<const uint32_t*>(&m);
+    } else {
+      const __nv_bfloat162 m =
+          __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&top), __habs2(*reinterpret_cast<__nv_bfloat162*>(&x)));
+      top = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  };
+#pragma unroll 2
+  for (int r = lo * 8 + (threadIdx.x & 31); r < hi * 8; r += 32)
+#pragma unroll
+    for (int h = 0; h < D / 64; ++h) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tile + h * pa::HALF + r * 16);
+      take(v.x);
+      take(v.y);
+      take(v.z);
+      take(v.w);
+    }
+  constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+  return __any_sync(0xffffffffu, (top & EXP) == EXP || (top >> 16 & EXP) == EXP) != 0;
+}
+
+// Takes them out of rows [lo, hi) of a value tile whose first key is `key` (one column per lane); returns the new base.
+// Not inlined, like all that is rare here: see mbar_wait_long.
+template <int D, bool F16>
+static __device__ __noinline__ int v_take_not_finite(uint8_t* tile, uint32_t* bad, int* s_base, int base, int key,
+                                                      int lo, int hi) {
+  const bool first = base < 0;
+  if (first) base = key;
+  constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+  for (int c = threadIdx.x & 31; c < D; c += 32) {
+    uint32_t e = first ? ALL_FINITE : bad[c];
+    for (int r = lo; r < hi; ++r) {
+      uint16_t* p = reinterpret_cast<uint16_t*>(tile + (c >> 6) * pa::HALF + r * 128 + (((c >> 3 & 7) ^ (r & 7)) << 4)) + (c & 7);
+      const uint32_t x = *p;
+      if ((x & EXP) != EXP) continue;
+      const int at = 10 * (x & (EXP ^ 0x7fff) ? 0 : x & 0x8000 ? 2 : 1);
+      if ((e >> at & NO_KEY) == NO_KEY) e ^= (NO_KEY ^ (uint32_t)(key - base + r)) << at;
+      *p = 0;
+    }
+    bad[c] = e;
+  }
+  *s_base = base;
+  fence_async_shared();
+  __syncwarp();
+  return base;
+}
+
+// What they add to a column of a row that sees `seen` keys from `base` on.
+LBW_DEV float not_finite_sum(uint32_t e, int seen) {
+  const bool nan = (int)(e & NO_KEY) < seen, up = (int)(e >> 10 & NO_KEY) < seen, down = (int)(e >> 20) < seen;
+  return nan || (up && down) ? __int_as_float(0x7fffffff) : up ? INFINITY : down ? -INFINITY : 0.f;
+}
+
+// Adds it to this thread's half of its row of the window, which the warp has just written.
+template <int D, bool F16>
+static __device__ __noinline__ void row_add_not_finite(const PackedArgs& a, const TileArgs& ta, const PackedWin& w,
+                                                       const uint32_t* bad, int base) {
+  const int warp = threadIdx.x >> 5, r0 = (warp & 3) * 32 + (threadIdx.x & 31), c0 = (warp >> 2 & 1) * (D / 2);
+  const int tok = w.tok[warp >> 3] + r0 / ta.pack, head = w.head0 + r0 % ta.pack;
+  __syncwarp();
+  if (r0 < ta.pack * ta.tile_toks && tok < w.sq.nq) {
+    const int seen = packed_visible(a, w.sq, tok) - base;
+    const long long row = (long long)w.sq.q0 + tok;
+    for (int c = c0; c < c0 + D / 2; ++c) {
+      const float x = not_finite_sum(bad[c], seen);
+      if (x == 0.f) continue;
+      if (ta.n_split > 1) {
+        ta.part_o[(((long long)w.split * a.tq + row) * a.hq + head) * D + c] += x;
+      } else {
+        uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + row * a.os_tok + head * a.os_head + c;
+        *p = (uint16_t)pack_16<F16>(unpack_16<F16>(*p) + x, 0.f);
+      }
+    }
+  }
+  __syncwarp();
+}
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(pa::THREADS, 1)
     packed_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -156,6 +248,8 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
   __shared__ PackedWin s_win[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ uint32_t s_bad[2][D];  // of window i in slot i & 1: values that are not finite
+  __shared__ int s_bad_base[2];     // their first key, -1: there are none
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -420,7 +514,14 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     bool ok = true;
     for (int i = 0; ok; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_c(&win_full[i & 1], (i >> 1) & 1, ab, 0x5f))) break;
-      const int n_p = s_win[i & 1].n_p, left = s_win[i & 1].sq.nk - s_win[i & 1].g0 * BN, valid = s_win[i & 1].valid;
+      const int n_p = s_win[i & 1].n_p, g0 = s_win[i & 1].g0, valid = s_win[i & 1].valid;
+      const int left = s_win[i & 1].sq.nk - g0 * BN;
+      // Keys that all rows of the pair see, and all rows of the primary alone (it goes on when the secondary has ended).
+      const int n_s = s_win[i & 1].n_s;
+      const int see_p = packed_visible(a, s_win[i & 1].sq, s_win[i & 1].tok[0]) - g0 * BN;
+      const int see_s = n_s > 0 ? packed_visible(a, s_win[i & 1].sq, s_win[i & 1].tok[1]) - g0 * BN : see_p;
+      int base = -1;  // (the softmax warps have left the slot's last window: it is this one's now)
+      if (lane == 0) s_bad_base[i & 1] = -1;
       __syncwarp();
       mbar_arrive_if(lane == 0, &win_empty[i & 1]);
       if (!valid) break;
@@ -437,6 +538,10 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
           fence_async_shared();
           __syncwarp();
         }
+        // Keys that some row does not see (what all see goes the usual way).
+        const int lo = max((j < n_s ? see_s : see_p) - j * BN, 0), hi = min(rows, BN);
+        if (lo < hi && v_not_finite<D, F16>(sV + s * TILE, lo, hi))
+          base = v_take_not_finite<D, F16>(sV + s * TILE, s_bad[i & 1], &s_bad_base[i & 1], base, (g0 + j) * BN, lo, hi);
         ok = j + 1 >= n_p || __all_sync(0xffffffffu, mbar_wait_c(&k_full[s ^ 1], ((jp + 1) >> 1) & 1, ab, 0x62));
         if (!ok) break;
         mbar_arrive_if(lane == 0, &p_ready[0]);
@@ -568,8 +673,11 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
       const int tok = w.tok[wg] + r0 / ta.pack, head = w.head0 + r0 % ta.pack, split = w.split;
       const bool mine = r0 < ta.pack * ta.tile_toks && tok < w.sq.nq && !abort_flag;
       const long long row = (long long)w.sq.q0 + tok;
+      // Values that are not finite and that this row sees (ordered by O's barrier behind the watcher's arrivals; what it
+      // writes for later tiles of the primary is of keys that the secondary's rows do not see).
+      const int base = n_tiles > 0 ? *(volatile int*)&s_bad_base[i & 1] : -1;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&win_empty[i & 1]);
+      if (lane == 0 && base < 0) mbar_arrive(&win_empty[i & 1]);
       if (ta.n_split > 1) {
         // unnormalised fp32 row and its (m, l); a row without a key leaves only l = 0
         const long long pr = ((long long)split * a.tq + row) * a.hq + head;
@@ -629,6 +737,10 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
           }
           __syncwarp();
         }
+      }
+      if (base >= 0) {
+        if (!abort_flag) row_add_not_finite<D, F16>(a, ta, s_win[i & 1], s_bad[i & 1], base);
+        if (lane == 0) mbar_arrive(&win_empty[i & 1]);
       }
     }
   }

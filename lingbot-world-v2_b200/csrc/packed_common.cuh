@@ -151,4 +151,13 @@ LBW_DEV uint32_t pack_16(float lo, float hi) {
   }
 }
 
+// The low 16 bits as a value.
+template <bool F16>
+LBW_DEV float unpack_16(uint32_t x) {
+  if constexpr (F16)
+    return __half2float(__ushort_as_half((unsigned short)x));
+  else
+    return __uint_as_float(x << 16);
+}
+
 }  // namespace lbw

@@ -266,6 +266,34 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][e] *= alpha[e >> 1];
       }
+      // Where rows do not see a key, its value must not reach them, and 0 * NaN would: such keys go by hand.
+      bool by_hand = false;
+      if (all_see < sq.nk && key0 + 16 > all_see) {
+        constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
+        for (int i = lane; i < 16 * D / 2; i += 32) {
+          const uint32_t x = *reinterpret_cast<const uint32_t*>(smem + s * 2 * TILE + TILE + i / 512 * HALF + kb * 128 + i % 512 * 4);
+          by_hand |= (x & EXP) == EXP || (x >> 16 & EXP) == EXP;
+        }
+        by_hand = __any_sync(0xffffffffu, by_hand);
+      }
+      if (by_hand) {
+#pragma unroll 1
+        for (int kk = 0; kk < 16; ++kk) {
+          const int key = kb + kk, from = (lane & ~3) | (kk >> 1 & 3);
+          const uint32_t w0 = __shfl_sync(0xffffffffu, kk < 8 ? p[0] : p[2], from) >> (kk & 1) * 16;
+          const uint32_t w1 = __shfl_sync(0xffffffffu, kk < 8 ? p[1] : p[3], from) >> (kk & 1) * 16;
+          const float p0 = unpack_16<F16>(w0), p1 = unpack_16<F16>(w1);
+          const bool in0 = key0 + kk < seen[0], in1 = key0 + kk < seen[1];
+#pragma unroll
+          for (int ch = 0; ch < D / 8; ++ch) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(smem + s * 2 * TILE + TILE + (ch >> 3) * HALF + key * 128 +
+                                                                  (((ch & 7) ^ (key & 7)) << 4) + c0 * 2);
+            const float v0 = unpack_16<F16>(x), v1 = unpack_16<F16>(x >> 16);
+            if (in0) o[ch][0] = fmaf(p0, v0, o[ch][0]), o[ch][1] = fmaf(p0, v1, o[ch][1]);
+            if (in1) o[ch][2] = fmaf(p1, v0, o[ch][2]), o[ch][3] = fmaf(p1, v1, o[ch][3]);
+          }
+        }
+      } else
 #pragma unroll
       for (int ch = 0; ch < D / 8; ch += 2) {
         uint32_t f[4];

@@ -1,4 +1,6 @@
 """Packed-sequence operators on a B200 against their 64-bit forms, every value within its own bound (packed_oracle)."""
+import math
+
 import pytest
 import torch
 
@@ -278,6 +280,43 @@ def test_packed_attention_nan_stays_with_its_sequence(cuda_dev):
         v[130 + 3] = float("inf")
         out = K.packed_attention(q, k, v, cu_q, cu_k)
         assert torch.isfinite(out[:lens[0]].float()).all() and torch.isfinite(out[last:].float()).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,q_lens,k_lens", [
+    ((4, 2), [300, 20], [300, 300]), ((6, 2), [130, 257], [200, 257]), ((4, 4), [200], [3000]),   # (keys in ranges)
+    ((2, 2), [1000, 700], [1000, 600]), ((4, 2), [5, 2, 1], [400, 131, 90]), ((1, 1), [16, 3], [16, 2]),
+    ((8, 2), list(range(1, 60)), list(range(1, 60)))])
+def test_packed_attention_values_that_are_not_finite(cuda_dev, heads, q_lens, k_lens, causal, dim, dtype):
+    """An infinite or NaN value makes its column of the rows that see it what the sum says, and changes nothing else."""
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, *heads, dim, dtype, qk_scale=0.5)
+    gen = torch.Generator().manual_seed(dim + len(q_lens))
+    n = 60
+    at = [torch.randint(0, hi, (n,), generator=gen) for hi in (v.shape[0], heads[1], dim)]
+    at[0][: n // 2] = v.shape[0] - 1 - torch.randint(0, min(150, v.shape[0]), (n // 2,), generator=gen)
+    kinds = torch.randint(0, 3, (n,), generator=gen)
+    at = tuple(at)
+    v[at] = 0
+    want, bound = po.attention(q, k, v, cu_q, cu_k, causal=causal)
+    add = torch.zeros(q.shape, dtype=torch.float64)
+    for row, head, col, kind in zip(*(x.tolist() for x in at), kinds.tolist()):
+        v[row, head, col] = (math.nan, math.inf, -math.inf)[kind]
+    group = heads[0] // heads[1]
+    for row, head, col in set(zip(*(x.tolist() for x in at))):
+        b = next(b for b in range(len(k_lens)) if row < sum(k_lens[:b + 1]))
+        key = row - sum(k_lens[:b])
+        first = max(0, key - (k_lens[b] - q_lens[b])) if causal else 0      # the first query that sees the key
+        rows = slice(sum(q_lens[:b]) + first, sum(q_lens[:b + 1]))
+        add[rows, head * group:(head + 1) * group, col] += float(v[row, head, col])
+    add = add.to(cuda_dev)
+    out = K.packed_attention(q, k, v, cu_q, cu_k, causal=causal).double()
+    hit = add != 0                                                          # (NaN too)
+    assert torch.equal(out[hit].isnan(), add[hit].isnan())
+    assert torch.equal(out[hit].nan_to_num(7.0, 1e9, -1e9), add[hit].nan_to_num(7.0, 1e9, -1e9))
+    assert po.within(out[~hit], want[~hit], bound[~hit]) <= 1
 
 
 def test_packed_attention_bad_starts_stay_inside(cuda_dev):
