@@ -12,10 +12,10 @@
 // mma.sync and not tcgen05: the rows of a unit fill an eighth of a 128-row tile, and 16 rows are enough to read at full
 // rate (a warp spends ~150 instructions on 16 keys = 8 KB; the SM's share of the memory rate is 23 bytes a clock).
 // Bound: the bytes of K and V. Measured (B200, bf16, 128-wide heads, 8 kv heads, both kernels, replayed from a graph):
-// 32 sequences of 16,384 keys 329 us with 1 row per kv head, 340 with 16 (6.5 and 6.3 TB/s: a plain copy's rate);
-// 128 x 500 keys 53 and 70 us (5.0 and 3.7 TB/s: a unit's join of its warps is not hidden behind 8 tiles of loads);
-// 1 x 30,000 keys 30 and 34 us (4.1 and 3.7 TB/s); 1 x 1,000 keys 8.5 and 10 us, which is two launches, the look-up of
-// the sequences and one trip to memory.
+// 32 sequences of 16,384 keys 326 us with 1 row per kv head, 336 with 16 (6.6 and 6.4 TB/s: a plain copy's rate);
+// 128 x 500 keys 50 and 59 us (5.3 and 4.4 TB/s: 7 units a CTA, whose ends - the join of 8 warps, masks, the next Q - are
+// not all hidden behind 8 tiles of loads); 1 x 30,000 keys 28 and 31 us (4.3 and 4.0 TB/s); 1 x 1,000 keys 8.2 and 10.4 us,
+// which is two launches, the look-up of the sequences and one trip to memory.
 #include "host_common.cuh"
 #include "packed_common.cuh"
 #include "packed_host.cuh"
@@ -172,6 +172,16 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
   // ---------------- consumers ----------------
   const int grp = warp >> 2, kb = (warp & 3) * 16;  // this warp's keys of a stage
   const int r_lo = lane >> 2, c0 = (lane & 3) * 2;
+  uint8_t* smem_q = reinterpret_cast<uint8_t*>(s_o);
+  const int q_row = threadIdx.x / (D / 8), q_chunk = threadIdx.x % (D / 8);
+  auto load_q = [&](const SplitUnit& w) {
+    const int row0 = w.unit / a.hk * ROWS, r = row0 + q_row;
+    if (q_row >= ROWS || r >= w.sq.nq * a.group) return make_uint4(0, 0, 0, 0);
+    const int tok = r / a.group, head = w.unit % a.hk * a.group + r - tok * a.group;
+    return *reinterpret_cast<const uint4*>(q + (long long)(w.sq.q0 + tok) * qs_tok + (long long)head * qs_head + q_chunk * 8);
+  };
+  uint4 q_piece;
+  bool have_q = false;
   int j = 0;
   for (long long g = first; g < last;) {
     const PackedSeq sq = u.sq;
@@ -179,20 +189,22 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
     if (n <= 0) break;  // as above; the same for all consumers, which follow one thread's reading
     const int head = u.unit % a.hk, row0 = u.unit / a.hk * ROWS;
     const int rows = min(sq.nq * a.group - row0, ROWS);
-    uint32_t qf[D / 16][4];
     int seen[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = r_lo + 8 * i;
-      const int tok = (row0 + r) / a.group;
-      seen[i] = r < rows ? packed_visible(a, sq, tok) : 0;
-      const uint16_t* src = q + (long long)(sq.q0 + tok) * qs_tok + (long long)(head * a.group + (row0 + r) % a.group) * qs_head;
+    for (int i = 0; i < 2; ++i)
+      seen[i] = r_lo + 8 * i < rows ? packed_visible(a, sq, (row0 + r_lo + 8 * i) / a.group) : 0;
+    // The unit's Q, a 16-byte piece per thread, through shared memory into the fragments of all warps (4-byte loads of 8
+    // rows at a time by every warp took 1 us of a unit's 9).
+    if (!have_q) q_piece = load_q(u);
+    if (q_row < ROWS) *reinterpret_cast<uint4*>(smem_q + q_row * D * 2 + ((q_chunk ^ (q_row & 7)) << 4)) = q_piece;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    uint32_t qf[D / 16][4];
 #pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        qf[s][i] = r < rows ? *reinterpret_cast<const uint32_t*>(src + s * 16 + c0) : 0u;
-        qf[s][i + 2] = r < rows ? *reinterpret_cast<const uint32_t*>(src + s * 16 + 8 + c0) : 0u;
-      }
+    for (int st = 0; st < D / 16; ++st) {
+      const int r = lane & 15, ch = st * 2 + (lane >> 4);
+      ldsm4(qf[st], smem_u32(smem_q) + r * D * 2 + ((ch ^ (r & 7)) << 4));
     }
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // (its place is the join's)
     const int all_see = packed_visible(a, sq, row0 / a.group);  // keys that every row of the unit sees
     float o[D / 8][4];
 #pragma unroll
@@ -270,10 +282,14 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
       bool by_hand = false;
       if (all_see < sq.nk && key0 + 16 > all_see) {
         constexpr uint32_t EXP = F16 ? 0x7c00u : 0x7f80u;
-        for (int i = lane; i < 16 * D / 2; i += 32) {
-          const uint32_t x = *reinterpret_cast<const uint32_t*>(smem + s * 2 * TILE + TILE + i / 512 * HALF + kb * 128 + i % 512 * 4);
-          by_hand |= (x & EXP) == EXP || (x >> 16 & EXP) == EXP;
-        }
+        for (int i = max(all_see - key0, 0) * 8 + lane; i < min(left, 16) * 8; i += 32)
+#pragma unroll
+          for (int h = 0; h < NH; ++h) {
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + s * 2 * TILE + TILE + h * HALF + kb * 128 + i * 16);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) by_hand |= (w[e] & EXP) == EXP || (w[e] >> 16 & EXP) == EXP;
+          }
         by_hand = __any_sync(0xffffffffu, by_hand);
       }
       if (by_hand) {
@@ -306,6 +322,13 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
       if (lane == 0) mbar_arrive(&empty[s]);
     }
 
+    // The next unit's Q is on its way during the join, if it is of the same sequence.
+    have_q = g + n < last && u.unit + 1 < u.units;
+    if (have_q) {
+      SplitUnit w = u;
+      ++w.unit;
+      q_piece = load_q(w);
+    }
     // The unit's end: join the 8 warps, 8 rows at a time.
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -318,9 +341,12 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (8 * i >= rows) break;
+      if (8 * i + r_lo < rows) {  // (8 columns' place turned by the row: the 8 rows of a store would be in the same banks)
 #pragma unroll
-      for (int ch = 0; ch < D / 8; ++ch)
-        *reinterpret_cast<float2*>(s_o + (warp * 8 + r_lo) * D + ch * 8 + c0) = make_float2(o[ch][2 * i], o[ch][2 * i + 1]);
+        for (int ch = 0; ch < D / 8; ++ch)
+          *reinterpret_cast<float2*>(s_o + (warp * 8 + r_lo) * D + (ch ^ r_lo) * 8 + c0) =
+              make_float2(o[ch][2 * i], o[ch][2 * i + 1]);
+      }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const int r = threadIdx.x >> 5;  // a warp per row, D / 32 values per lane
       if (8 * i + r < rows) {
@@ -335,7 +361,7 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
           const float k = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
           L += k * ml.y;
 #pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] += k * s_o[(w * 8 + r) * D + lane * PER + e];
+          for (int e = 0; e < PER; ++e) acc[e] += k * s_o[(w * 8 + r) * D + ((lane * PER) ^ (r * 8)) + e];
         }
         if (begins && ends) {
           const int tok = (row0 + 8 * i + r) / a.group, hh = head * a.group + (row0 + 8 * i + r) % a.group;
