@@ -249,14 +249,8 @@ typedef struct {
   unsigned char axis[128];
   unsigned long long step[128];
 } lbw_rope_axes;
-/* out = x rotated, fp32 arithmetic, one rounding; dims beyond 2 * pairs are copied. x, out: [tokens, heads, head_dim]
- * of lbw_dtype `dtype` (head_dim a multiple of 8, at most 256; out may be x). positions: [tokens, axes] int32 or int64
- * (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does nothing. */
-int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, long long out_tok, long long out_head,
-                   long long tokens, int heads, int head_dim, int dtype, const void* positions, int pos_bits,
-                   long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream);
-/* One operand of lbw_qk_headnorm_rope: x [tokens, heads, head_dim] -> out [rows, heads, head_dim]; gamma [head_dim]
- * of the tensors' type (or fp32 with gamma_f32), or NULL for no gain. */
+/* An operand of the row kernels: x [tokens, heads, head_dim] -> out [rows, heads, head_dim]; gamma [head_dim] of the
+ * tensors' type (or fp32 with gamma_f32), or NULL for no gain. */
 typedef struct {
   const void* x;
   void* out;
@@ -264,6 +258,11 @@ typedef struct {
   long long x_tok, x_head, out_row, out_head;
   int heads, gamma_f32;
 } lbw_head_rows;
+/* out = x rotated, fp32 arithmetic, one rounding; dims beyond 2 * pairs are copied (x->gamma is not used). lbw_dtype
+ * `dtype`, head_dim a multiple of 8, at most 256; out may be x, with the same strides. positions: [tokens, axes] int32 or
+ * int64 (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does nothing. */
+int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int dtype, const void* positions, int pos_bits,
+                   long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream);
 /* Every head vector of q and k: x * rsqrt(mean(x^2) + eps) * gamma, then the rotation (rope NULL: none), fp32 with one
  * rounding. With k_rows (int32 or int64 [tokens], k_rows_bits) token t's k goes to row k_rows[t] of k->out, and v, if
  * given, is copied to row k_rows[t] of v->out (a cache of out_rows rows); a row outside [0, out_rows) is not written.
@@ -275,6 +274,20 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
                          long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
                          long long out_rows, void* stream);
 
+typedef struct {
+  const void* q;
+  long long q_tok, q_head;
+  const void* k;
+  long long k_tok, k_head;
+  const void* v;
+  long long v_tok, v_head;
+  void* out;
+  long long out_tok, out_head;
+  const int *cu_q, *cu_k, *k_lens;
+  long long tq, tk;
+  int n_seqs, hq, hk, head_dim, dtype, causal, max_q;
+  float softmax_scale;
+} lbw_packed_batch;
 /* Attention of a batch of packed sequences: out_i = sum_j p_ij v_j with p = softmax over the visible keys of
  * softmax_scale * q_i k_j, fp32 scores and sums. Sequence b has the query rows cu_q[b] .. cu_q[b + 1] - 1 and the keys
  * cu_k[b] ..; there are cu_k[b + 1] - cu_k[b] of them, or k_lens[b] if k_lens is given (a cache with room for more: the
@@ -291,11 +304,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
  * that such a call enqueues). out may be q, with the same strides. */
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
                                    int same_lens, long long* bytes, int* launches);
-int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const void* k, long long k_tok,
-                         long long k_head, const void* v, long long v_tok, long long v_head, void* out,
-                         long long out_tok, long long out_head, const int* cu_q, const int* cu_k, const int* k_lens,
-                         int n_seqs, long long tq, long long tk, int hq, int hk, int head_dim, int dtype, int causal,
-                         float softmax_scale, int max_q, void* workspace, long long ws_bytes, void* stream);
+int lbw_packed_attention(const lbw_packed_batch* batch, void* workspace, long long ws_bytes, void* stream);
 
 /* ---- MXFP8 -------------------------------------------------------------------------------- */
 /* Quantise bf16 x [rows, k] (k % 128 == 0) to E4M3 data [rows, k] and E8M0 scales in the tiled

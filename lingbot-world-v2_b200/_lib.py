@@ -67,11 +67,10 @@ SIGNATURES = {
     "lbw_mx_linear_rowss": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp], _i),
     "lbw_mx_linear_residual_film": ([_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp], _i),
     "lbw_mx_linear_act": ([_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp], _i),
-    "lbw_axial_rope": ([_vp, _ll, _ll, _vp, _ll, _ll, _ll, _i, _i, _i, _vp, _i, _ll, _ll, _vp, _i, _vp], _i),
+    "lbw_axial_rope": ([_vp, _ll, _i, _i, _vp, _i, _ll, _ll, _vp, _i, _vp], _i),
     "lbw_qk_headnorm_rope": ([_vp, _vp, _vp, _ll, _i, _i, _f, _vp, _i, _ll, _ll, _vp, _vp, _i, _ll, _vp], _i),
     "lbw_packed_attention_workspace": ([_ll, _ll, _i, _i, _i, _i, _i, _i, ctypes.POINTER(_ll), ctypes.POINTER(_i)], _i),
-    "lbw_packed_attention": ([_vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _vp, _i, _ll, _ll,
-                              _i, _i, _i, _i, _i, _f, _i, _vp, _ll, _vp], _i),
+    "lbw_packed_attention": ([_vp, _vp, _ll, _vp], _i),
     "lbw_vae_conv": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp], _i),
     "lbw_vae_conv_rms": ([_vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp], _i),
     "lbw_vae_rms_silu": ([_vp, _ll, _i, _i, _vp, _i, _vp, _vp], _i),
@@ -148,6 +147,7 @@ def check(rc, what, launches=1):
 
 # lbw_head_rows (include/lbw.h) as bytes: x, out, gamma, x_tok, x_head, out_row, out_head, heads, gamma_f32.
 HEAD_ROWS = struct.Struct("@PPPqqqqii")
+PACKED_BATCH = struct.Struct("@PqqPqqPqqPqqPPPqqiiiiiiif")   # lbw_packed_batch
 
 
 def ptr(t):

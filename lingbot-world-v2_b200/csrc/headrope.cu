@@ -283,13 +283,12 @@ __global__ void __launch_bounds__(hr::THREADS, hr::MINB) head_rope_kernel(const 
 
 using namespace lbw;
 
-// Checks one segment's pointers and strides; `elem` bytes per value.
-static int check_seg(const char* who, const char* name, const void* x, const void* out, long long xs_tok,
-                     long long xs_head, long long os_tok, long long os_head, int heads, int elem) {
-  if (!x || !out) return set_error(LBW_ERR_INVALID, "%s: null %s", who, name);
-  if (heads < 1 || heads > 1 << 20) return set_error(LBW_ERR_SHAPE, "%s: %d %s heads", who, heads, name);
-  const long long per = 16 / elem;
-  if (!aligned(x, 16) || !aligned(out, 16) || xs_tok % per || xs_head % per || os_tok % per || os_head % per)
+// Checks one operand's pointers and strides.
+static int check_seg(const char* who, const char* name, const lbw_head_rows& r, int dtype) {
+  if (!r.x || !r.out) return set_error(LBW_ERR_INVALID, "%s: null %s", who, name);
+  if (r.heads < 1 || r.heads > 1 << 20) return set_error(LBW_ERR_SHAPE, "%s: %d %s heads", who, r.heads, name);
+  const long long per = dtype == LBW_FP32 ? 4 : 8;
+  if (!aligned(r.x, 16) || !aligned(r.out, 16) || r.x_tok % per || r.x_head % per || r.out_row % per || r.out_head % per)
     return set_error(LBW_ERR_ALIGN, "%s: %s needs 16-byte aligned pointers and strides", who, name);
   return LBW_OK;
 }
@@ -375,18 +374,16 @@ static int launch_head_rope(HeadArgs& a, int dtype, cudaStream_t s, const char* 
 
 extern "C" {
 
-int lbw_axial_rope(const void* x, long long x_tok, long long x_head, void* out, long long out_tok, long long out_head,
-                   long long tokens, int heads, int head_dim, int dtype, const void* positions, int pos_bits,
+int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int dtype, const void* positions, int pos_bits,
                    long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream) {
   const char* who = "axial_rope";
-  if (!rope) return set_error(LBW_ERR_INVALID, "%s: null rope", who);
+  if (!x || !rope) return set_error(LBW_ERR_INVALID, "%s: null %s", who, x ? "rope" : "x");
   int err = check_common(who, tokens, head_dim, dtype, positions, pos_bits, rope);
   if (err) return err;
   if (tokens == 0) return LBW_OK;
-  if ((err = check_seg(who, "x", x, out, x_tok, x_head, out_tok, out_head, heads, dtype == LBW_FP32 ? 4 : 2)))
-    return err;
+  if ((err = check_seg(who, "x", *x, dtype))) return err;
   HeadArgs a{};
-  a.seg[0] = HeadSeg{x, out, nullptr, x_tok, x_head, out_tok, out_head, heads, 0};
+  a.seg[0] = HeadSeg{x->x, x->out, nullptr, x->x_tok, x->x_head, x->out_row, x->out_head, x->heads, 0};
   if ((err = check_in_place(who, a.seg[0], tokens, false))) return err;
   a.tokens = tokens;
   a.dim = head_dim;
@@ -419,9 +416,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
   for (int i = 0; i < 3; ++i) {
     if (!in[i]) continue;
     const lbw_head_rows& r = *in[i];
-    if ((err = check_seg(who, names[i], r.x, r.out, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads,
-                         dtype == LBW_FP32 ? 4 : 2)))
-      return err;
+    if ((err = check_seg(who, names[i], r, dtype))) return err;
     if (r.gamma && !aligned(r.gamma, r.gamma_f32 ? 4 : 2))
       return set_error(LBW_ERR_ALIGN, "%s: gamma of %s is misaligned", who, names[i]);
     a.seg[i] = HeadSeg{r.x, r.out, r.gamma, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads, r.gamma_f32};

@@ -912,11 +912,10 @@ int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, i
   return LBW_OK;
 }
 
-int lbw_packed_attention(const void* q, long long q_tok, long long q_head, const void* k, long long k_tok,
-                         long long k_head, const void* v, long long v_tok, long long v_head, void* out,
-                         long long out_tok, long long out_head, const int* cu_q, const int* cu_k, const int* k_lens,
-                         int n_seqs, long long tq, long long tk, int hq, int hk, int head_dim, int dtype, int causal,
-                         float softmax_scale, int max_q, void* workspace, long long ws_bytes, void* stream) {
+int lbw_packed_attention(const lbw_packed_batch* batch, void* workspace, long long ws_bytes, void* stream) {
+  if (!batch) return set_error(LBW_ERR_INVALID, "packed_attention: null batch");
+  const auto& [q, q_tok, q_head, k, k_tok, k_head, v, v_tok, v_head, out, out_tok, out_head, cu_q, cu_k, k_lens, tq, tk,
+               n_seqs, hq, hk, head_dim, dtype, causal, max_q, softmax_scale] = *batch;
   const char* who = "packed_attention";
   int err = check_packed(tq, tk, hq, hk, head_dim, n_seqs);
   if (err) return err;

@@ -11,7 +11,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import HEAD_ROWS, check, load, ptr, raw_stream, require_cuda, stream_of
+from ._lib import HEAD_ROWS, PACKED_BATCH, check, load, ptr, raw_stream, require_cuda, stream_of
 
 BF16 = torch.bfloat16
 HEAD_DIM = 128
@@ -830,8 +830,9 @@ def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
     if o_tokens != tokens or o_heads != heads:
         raise ValueError(f"{who}: out is {tuple(out.shape)}, x {tuple(x.shape)}")
     pos = _positions(who, positions, tokens, rope)
-    check(_launch(dev, load().lbw_axial_rope, x.data_ptr(), x_tok, x_head, out.data_ptr(), o_tok, o_head, tokens, heads,
-                  dim, DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0), who, launches=1 if tokens else 0)
+    seg = HEAD_ROWS.pack(x.data_ptr(), out.data_ptr(), 0, x_tok, x_head, o_tok, o_head, heads, 0)
+    check(_launch(dev, load().lbw_axial_rope, seg, tokens, dim, DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0), who,
+          launches=1 if tokens else 0)
     return out
 
 
@@ -925,7 +926,7 @@ def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=N
     same_lens: for calls with one tensor as cu_q and cu_k and no k_lens."""
     device = torch.device(device)
     dev = torch.cuda.current_device() if device.index is None else device.index
-    n, _ = _packed_attention_plan(tq, tk, hq, hk, head_dim, n_seqs, int(max_q or 0), bool(same_lens), dev)
+    n, _ = _packed_attention_plan(tq, tk, hq, hk, head_dim, n_seqs, min(int(max_q or 0), tq), bool(same_lens), dev)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
@@ -964,6 +965,8 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
         max_q = 0
     elif max_q < 0:
         raise ValueError(f"{who}: max_q {max_q}")
+    elif max_q > tq:
+        max_q = tq
     if out is None:
         out = torch.empty_like(q)
     o_rows, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
@@ -978,9 +981,9 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
         ws_bytes = workspace.numel() * workspace.element_size()
     elif ws_bytes:
         workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
-    check(_launch(dev, load().lbw_packed_attention, q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head,
-                  v.data_ptr(), v_tok, v_head, out.data_ptr(), o_tok, o_head, pq, pk,
-                  None if k_lens is None else k_lens.data_ptr(), n, tq, tk, hq, hk, dim, DTYPES[dtype],
-                  1 if causal else 0, scale, max_q, None if workspace is None else workspace.data_ptr(), ws_bytes), who,
-          launches=launches)
+    batch = PACKED_BATCH.pack(q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head,
+                              out.data_ptr(), o_tok, o_head, pq, pk, 0 if k_lens is None else k_lens.data_ptr(), tq, tk,
+                              n, hq, hk, dim, DTYPES[dtype], 1 if causal else 0, max_q, scale)
+    check(_launch(dev, load().lbw_packed_attention, batch, None if workspace is None else workspace.data_ptr(), ws_bytes),
+          who, launches=launches)
     return out

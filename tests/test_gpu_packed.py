@@ -365,7 +365,7 @@ def test_packed_attention_over_many_short_sequences(cuda_dev):
     q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, 4, 2, 64, BF)
     want, bound = po.attention(q, k, v, cu_q, cu_k)
     assert po.within(K.packed_attention(q, k, v, cu_q, cu_k), want, bound) <= 1
-    for lens in (None, 70):
+    for lens in (None, 70, 1 << 40):
         x = q.clone()
         assert K.packed_attention(x, k, v, cu_q, cu_k, out=x, max_q=lens) is x
         assert po.within(x, want, bound) <= 1

@@ -57,6 +57,23 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def _axial(lib, a):
+    seg = L.HEAD_ROWS.pack(_at(a["x"]), _at(a["out"]), 0, a["x_tok"], a["x_head"], a["out_tok"], a["out_head"], a["heads"], 0)
+    return lib.lbw_axial_rope(seg, *(a[n] for n in ("tokens", "dim", "dtype", "pos", "bits", "pos_tok", "pos_axis", "rope",
+                                                    "inverse")), None)
+
+
+def _packed(lib, a):
+    first = "q q_tok q_head k k_tok k_head v v_tok v_head out out_tok out_head cu_q cu_k k_lens".split()
+    batch = L.PACKED_BATCH.pack(*(_at(a[n]) for n in first), *(a[n] for n in ("tq", "tk", "n", "hq", "hk", "dim", "dtype",
+                                                                            "causal", "max_q", "scale")))
+    return lib.lbw_packed_attention(batch, a["ws"], a["ws_bytes"], None)
+
+
+def _at(p):
+    return (p.value if isinstance(p, ctypes.c_void_p) else p) or 0
+
+
 def _rope(pairs=32, axes=1, layout=0, axis=0):
     r = rope.RopeAxes(pairs, axes, layout, 0)
     r.axis[0] = axis
@@ -79,7 +96,7 @@ def test_axial_rope_entry_checks(lib, change, status):
     a = dict(x=P, x_tok=1024, x_head=64, out=P, out_tok=1024, out_head=64, tokens=5, heads=2, dim=64, dtype=0, pos=P,
              bits=32, pos_tok=1, pos_axis=1, rope=_rope(), inverse=0)
     a.update(change)
-    rc = lib.lbw_axial_rope(*a.values(), None)
+    rc = _axial(lib, a)
     assert rc == status
     if status:
         assert "axial_rope" in L.last_error()
@@ -104,6 +121,11 @@ def test_qk_headnorm_rope_entry_checks(lib, change, status):
     assert lib.lbw_qk_headnorm_rope(*a.values(), None) == status
 
 
+CALL = dict(q=P, q_tok=1024, q_head=64, k=P, k_tok=1024, k_head=64, v=P, v_tok=1024, v_head=64, out=P, out_tok=1024,
+            out_head=64, cu_q=P, cu_k=P, k_lens=None, n=2, tq=100, tk=100, hq=8, hk=2, dim=64, dtype=0, causal=1, scale=0.1,
+            max_q=0, ws=P, ws_bytes=1 << 40)
+
+
 @pytest.mark.parametrize("change,status", [
     (dict(q=None), L.LBW_ERR_INVALID), (dict(v=None), L.LBW_ERR_INVALID), (dict(out=None), L.LBW_ERR_INVALID),
     (dict(cu_q=None), L.LBW_ERR_INVALID), (dict(dim=96), L.LBW_ERR_SHAPE), (dict(hk=3), L.LBW_ERR_SHAPE),
@@ -113,44 +135,40 @@ def test_qk_headnorm_rope_entry_checks(lib, change, status):
     (dict(out=ctypes.c_void_p(4104)), L.LBW_ERR_ALIGN), (dict(cu_k=ctypes.c_void_p(4098)), L.LBW_ERR_ALIGN),
     (dict(tq=0), L.LBW_OK), (dict(n=0), L.LBW_OK)])
 def test_packed_attention_entry_checks(lib, change, status):
-    a = dict(q=P, q_tok=1024, q_head=64, k=P, k_tok=1024, k_head=64, v=P, v_tok=1024, v_head=64, out=P, out_tok=1024,
-             out_head=64, cu_q=P, cu_k=P, k_lens=None, n=2, tq=100, tk=100, hq=8, hk=2, dim=64, dtype=0, causal=1,
-             scale=0.1, max_q=0, ws=P, ws_bytes=1 << 40)
-    a.update(change)
-    assert lib.lbw_packed_attention(*a.values(), None) == status
+    assert _packed(lib, {**CALL, **change}) == status
 
 
 def test_packed_attention_refuses_a_small_workspace(lib):
     n = ctypes.c_longlong(-1)
     assert lib.lbw_packed_attention_workspace(1, 100000, 8, 2, 128, 1, 1, 0, ctypes.byref(n), None) == L.LBW_OK
     assert n.value > 0
-    rc = lib.lbw_packed_attention(P, 1024, 128, P, 1024, 128, P, 1024, 128, P, 1024, 128, P, P, None, 1, 1, 100000, 8, 2,
-                                  128, 0, 1, 0.1, 1, P, n.value - 1, None)
+    rc = _packed(lib, {**CALL, "q_head": 128, "k_head": 128, "v_head": 128, "out_head": 128, "n": 1, "tq": 1, "tk": 100000,
+                       "dim": 128, "max_q": 1, "ws_bytes": n.value - 1})
     assert rc == L.LBW_ERR_INVALID and "workspace" in L.last_error()
     assert lib.lbw_packed_attention_workspace(1, 100, 8, 3, 128, 1, 1, 0, ctypes.byref(n), None) == L.LBW_ERR_SHAPE
     assert lib.lbw_packed_attention_workspace(1, 100, 8, 2, 128, 1, 1, 0, None, None) == L.LBW_ERR_INVALID
+    assert lib.lbw_packed_attention(None, P, 0, None) == lib.lbw_axial_rope(None, 1, 64, 0, P, 32, 1, 1, _rope(), 0, None) \
+        == L.LBW_ERR_INVALID
 
 
 def test_in_place_calls_that_would_race_are_refused(lib):
     """x as its own output with other strides or rows, keys or values as the output of the attention."""
     axial = dict(x=P, x_tok=1024, x_head=64, out=P, out_tok=2048, out_head=64, tokens=5, heads=2, dim=64, dtype=0, pos=P,
                  bits=32, pos_tok=1, pos_axis=1, rope=_rope(), inverse=0)
-    assert lib.lbw_axial_rope(*axial.values(), None) == L.LBW_ERR_INVALID and "in place" in L.last_error()
+    assert _axial(lib, axial) == L.LBW_ERR_INVALID and "in place" in L.last_error()
     there = _rows(out=8192)
     for q, k, v, rows in ((_rows(out_head=128), there, None, None), (there, _rows(), None, P), (there, there, _rows(), P)):
         assert lib.lbw_qk_headnorm_rope(q, k, v, 5, 64, 0, 1e-6, P, 32, 1, 1, _rope(), rows, 64, 9, None) == L.LBW_ERR_INVALID
         assert "in place" in L.last_error()
     far = ctypes.c_void_p(1 << 20)
     for q, k, v, out_tok in ((far, P, far, 1024), (far, far, P, 1024), (P, far, far, 2048)):
-        assert lib.lbw_packed_attention(q, 1024, 64, k, 1024, 64, v, 1024, 64, P, out_tok, 64, P, P, None, 2, 100, 100, 8, 2,
-                                        64, 0, 1, 0.1, 0, P, 1 << 40, None) == L.LBW_ERR_INVALID
+        assert _packed(lib, {**CALL, "q": q, "k": k, "v": v, "out_tok": out_tok}) == L.LBW_ERR_INVALID
         assert "out is" in L.last_error()
 
 
 def test_packed_attention_refuses_a_scale_out_of_range(lib):
     for scale in (3e38, 1e-46):                                             # times log2 e: infinite, zero
-        assert lib.lbw_packed_attention(P, 1024, 64, P, 1024, 64, P, 1024, 64, P, 1024, 64, P, P, None, 2, 100, 100, 8, 2,
-                                        64, 0, 1, scale, 0, P, 1 << 40, None) == L.LBW_ERR_INVALID
+        assert _packed(lib, {**CALL, "scale": scale}) == L.LBW_ERR_INVALID
         assert "softmax_scale" in L.last_error()
 
 
