@@ -57,29 +57,53 @@ struct TileArgs {
   float* part_ml;  // [n_split][tq * hq][2]
 };
 
-// tcgen05 operations of a converged warp, issued by the lanes with lead != 0 (one of them).
-LBW_DEV void mma_f16_ss_if(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
-      : "memory");
+// tcgen05 operations of a converged warp, issued by one of its lanes. Which: for D = 128 the elected one (always the same),
+// elected in each operation's own asm; for D = 64 lane 0, by the predicate `lead`. A predicated MMA takes the issuer 79
+// cycles, an elected one 65, and one runs for 64 (32 where D = 64 is its N). Measured (us, elected / predicated): D = 128
+// 10,800 causal tokens 1,032 / 1,070, 64 x 300..900 359 / 372; D = 64 16,000 tokens 1,545 / 1,405, 8 x 1,000 63 / 59.
+template <bool ELECT>
+LBW_DEV void mma_f16_ss_one(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  if constexpr (ELECT)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
 }
-LBW_DEV void mma_f16_ts_if(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
-      : "memory");
+template <bool ELECT>
+LBW_DEV void mma_f16_ts_one(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  if constexpr (ELECT)
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
 }
-LBW_DEV void tc_commit_if(uint32_t lead, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
-      "r"(lead)
-      : "memory");
+template <bool ELECT>
+LBW_DEV void tc_commit_one(uint32_t lead, uint64_t* bar) {
+  if constexpr (ELECT)
+    asm volatile(
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar))
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(lead)
+        : "memory");
 }
 
 // One window: the key range [g0, g0 + n_p) (in 128-key tiles) of a pair of query tiles.
@@ -433,8 +457,9 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     // ---------------- MMA issuer ----------------
     // MMAs execute in issue order: S of a window's first tile may be issued right behind the last P V of the window
     // before, and its O is overwritten only by a P V that waits for a P written after that O was read.
-    // The whole warp runs this code and lane 0 issues (by predicate): in a branch of one lane every descriptor would have to
-    // be moved to the uniform registers that the MMA reads.
+    // The whole warp runs this code and one lane issues (by predicate): in a branch of one lane every descriptor would have
+    // to be moved to the uniform registers that the MMA reads.
+    constexpr bool ELECT = D == 128;
     const uint32_t lead = lane == 0;
     const uint32_t idesc_s = F16 ? idesc_f16(BM, BN, 0, 0) : idesc_bf16(BM, BN, 0, 0);  // S = Q K^T, both K-major
     const uint32_t idesc_o = F16 ? idesc_f16(BM, D, 0, 1) : idesc_bf16(BM, D, 0, 1);    // O += P V, V MN-major
@@ -447,14 +472,14 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
         const uint64_t off = (uint64_t)(((kk >> 2) * HALF + (kk & 3) * 32) >> 4);
-        mma_f16_ss_if(lead, tm + i * 128, q + off, k + off, idesc_s, kk > 0);
+        mma_f16_ss_one<ELECT>(lead, tm + i * 128, q + off, k + off, idesc_s, kk > 0);
       }
     };
     auto issue_pv = [&](int i, int stage, bool first) {
       const uint64_t v = dV + (uint64_t)((stage * TILE) >> 4);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk)  // P of keys 64.. lies over its own scores, 64 columns on
-        mma_f16_ts_if(lead, tm + 256 + i * D, tm + i * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
+        mma_f16_ts_one<ELECT>(lead, tm + 256 + i * D, tm + i * 128 + (kk >> 2) * 64 + (kk & 3) * 8,
                       v + (uint64_t)((kk * 2048) >> 4), idesc_o, !(first && kk == 0));
     };
     auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
@@ -466,7 +491,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
       if (!wait(&win_full[i & 1], (i >> 1) & 1, 0x30)) break;
       const int n_p = __shfl_sync(0xffffffffu, s_win[i & 1].n_p, 0), n_s = __shfl_sync(0xffffffffu, s_win[i & 1].n_s, 0);
       const int valid = __shfl_sync(0xffffffffu, s_win[i & 1].valid, 0);
-      if (lead) mbar_arrive(&win_empty[i & 1]);
+      mbar_arrive_if(lead, &win_empty[i & 1]);
       if (!valid) break;
       if (n_p == 0) continue;
       if (!wait(&q_full, nq_loads & 1, 0x31) || !wait(&k_full[jp & 1], (jp >> 1) & 1, 0x32)) break;
@@ -479,28 +504,28 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int n = t ? n_s : n_p;
-          if (t && j >= 0 && (j >= n || !ok)) tc_commit_if(lead, &v_empty[s]);
+          if (t && j >= 0 && (j >= n || !ok)) tc_commit_one<ELECT>(lead, &v_empty[s]);
           if (j >= n || !ok) continue;
           if (j >= 0) {
             if (!(ok = wait(&p_ready[t], (t ? js : jp) & 1, 0x34 + t))) continue;
             tc_fence_after();
             issue_pv(t, s, j == 0);
             js += t;
-            if (t) tc_commit_if(lead, &v_empty[s]);
+            if (t) tc_commit_one<ELECT>(lead, &v_empty[s]);
           }
           if (j + 1 < n) {
             issue_s(t, s1);
-            tc_commit_if(lead, &s_full[t]);
+            tc_commit_one<ELECT>(lead, &s_full[t]);
           } else if (n > 0) {
-            tc_commit_if(lead, &o_done[t]);
+            tc_commit_one<ELECT>(lead, &o_done[t]);
           }
         }
-        if (j + 1 < n_p) tc_commit_if(lead, &k_empty[s1]);
-        if (j + 2 == n_p) tc_commit_if(lead, &q_empty);  // the window's last S has been issued
+        if (j + 1 < n_p) tc_commit_one<ELECT>(lead, &k_empty[s1]);
+        if (j + 2 == n_p) tc_commit_one<ELECT>(lead, &q_empty);  // the window's last S has been issued
         jp += j >= 0;
       }
     }
-    tc_commit_if(lead, &done_bar);
+    tc_commit_one<ELECT>(lead, &done_bar);
     mbar_wait_drain(&done_bar, 0);
   } else if (warp == 18) {
     // ---------------- K/V watcher ----------------
