@@ -29,6 +29,10 @@
 // tile. Tried and slower: exponentials on the FMA pipe (1/8 to 1/2 of them, +1 to +5%), an issuer per tile (+4 to +20%),
 // one thread per row and two P releases (+10%), P beside S for D = 64 (-8% for long sequences, +10% for short ones), the
 // maximum of the tile before as m (+5%), rolled MMA loops (+8%), waits of one lane (+17%) or with a suspend hint (+7%).
+// Windows of one or two key tiles take ~9,000 cycles, softmax 2,500, P V 850, rows written 3,300: each role's code comes
+// from beyond the instruction cache again in every window (390 misses, some 50 KB). Tried for them: a rolled loop over the
+// two tiles in the issuer (-4 to -10%, but +3% for long sequences), the next window's first S behind the last P V (+1%), a
+// run of the issuer's code without effect ahead of time (+5 to +10%), the softmax in halves (-1%, long +8%).
 // Rows that see no key (causal with fewer keys than queries, no keys at all) get zeros.
 #include <limits.h>
 
@@ -274,6 +278,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
   __shared__ int abort_flag;
   __shared__ uint32_t s_bad[2][D];  // of window i in slot i & 1: values that are not finite
   __shared__ int s_bad_base[2];     // their first key, -1: there are none
+  __shared__ int s_rank[32];        // the scheduler's
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -350,6 +355,23 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
           if (loaded != b_at) {  // 32 sequences, one per lane, kept while windows come from them
             const int b = b_at + lane;
             s = b < a.n_seqs ? packed_seq(a, b) : PackedSeq{0, 0, 0, 0};
+            if (a.n_seqs > 1) {
+              // Those with most keys first: their windows are the longest, and a CTA that took one last would be alone.
+              int rank = 0;
+#pragma unroll
+              for (int o = 0; o < 32; ++o) {
+                const int nk = __shfl_sync(0xffffffffu, s.nk, o);
+                rank += nk > s.nk || (nk == s.nk && o < lane);
+              }
+              s_rank[rank] = lane;
+              __syncwarp();
+              const int from = s_rank[lane];
+              s.q0 = __shfl_sync(0xffffffffu, s.q0, from);
+              s.nq = __shfl_sync(0xffffffffu, s.nq, from);
+              s.k0 = __shfl_sync(0xffffffffu, s.k0, from);
+              s.nk = __shfl_sync(0xffffffffu, s.nk, from);
+              __syncwarp();
+            }
             own = (long long)s.nq * a.group <= ta.short_rows ? 0 : (s.nq + 2 * ta.tile_toks - 1) / (2 * ta.tile_toks);
             upto = own;
 #pragma unroll
