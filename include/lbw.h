@@ -266,9 +266,9 @@ int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int d
 /* Every head vector of q and k: x * rsqrt(mean(x^2) + eps) * gamma, then the rotation (rope NULL: none), fp32 with one
  * rounding. With k_rows (int32 or int64 [tokens], k_rows_bits) token t's k goes to row k_rows[t] of k->out, and v, if
  * given, is copied to row k_rows[t] of v->out (a cache of out_rows rows); a row outside [0, out_rows) is not written.
- * Without k_rows the rows are the tokens. Two tokens with the same row leave a mix of both
- * there. The sums of squares are fp32: values beyond 1e18 make them infinite and the head zero. out may be x (k and v:
- * without k_rows), with the same strides. */
+ * Without k_rows the rows are the tokens. Two tokens with the same row leave a mix of both there. The sums of squares are
+ * fp32: values beyond 1e18 make them infinite and the head zero. out may be x (k: without k_rows), with the same
+ * strides. */
 int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
                          int head_dim, int dtype, float eps, const void* positions, int pos_bits, long long pos_tok,
                          long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
@@ -295,9 +295,10 @@ typedef struct {
  * 0 .. i + nk - nq. A row that sees no key gets zeros; rows of no sequence are left alone. cu_q, cu_k, k_lens: device
  * int32, read when the kernels run (a captured graph may be replayed with others); starts and lengths that do not fit
  * the tensors are cut to what does.
- * q, out: [tq, hq, head_dim]; k, v: [tk, hk, head_dim]; hq a multiple of hk, query head h uses kv head h / (hq / hk);
- * head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A value that is not finite makes its column infinite or NaN
- * in the rows that see it, a NaN key all of such a row; no other row is touched.
+ * q, out: [tq, hq, head_dim]; k, v: [tk, hk, head_dim]; hq (at most 65,536) a multiple of hk, query head h uses kv head
+ * h / (hq / hk); tq * hq and tk below 2^31 - 1,024; head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A value
+ * that is not finite makes its column infinite or NaN in the rows that see it, a NaN key all of such a row; no other row
+ * is touched.
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
  * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
  * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels

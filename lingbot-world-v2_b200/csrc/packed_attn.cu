@@ -939,9 +939,10 @@ static int check_packed(long long tq, long long tk, int hq, int hk, int d, int n
   if (d != 64 && d != 128) return set_error(LBW_ERR_SHAPE, "%s: head_dim %d (64 or 128)", who, d);
   if (hk < 1 || hq < hk || hq % hk || hq > 65536)
     return set_error(LBW_ERR_SHAPE, "%s: %d query heads over %d kv heads", who, hq, hk);
-  if (tq < 0 || tk < 0 || tq >= 1ll << 31 || tk >= 1ll << 31)
-    return set_error(LBW_ERR_SHAPE, "%s: %lld query rows, %lld key rows", who, tq, tk);
-  if (n_seqs < 0) return set_error(LBW_ERR_SHAPE, "%s: %d sequences", who, n_seqs);
+  // (Below 2^31 with room for a tile: rows and their products with heads are 32-bit in the kernels.)
+  if (tq < 0 || tq >= 1ll << 31 || tk < 0 || tq * hq >= (1ll << 31) - 1024 || tk >= (1ll << 31) - 1024)
+    return set_error(LBW_ERR_SHAPE, "%s: %lld query rows of %d heads, %lld key rows", who, tq, hq, tk);
+  if (n_seqs < 0 || n_seqs >= 1 << 30) return set_error(LBW_ERR_SHAPE, "%s: %d sequences", who, n_seqs);
   return LBW_OK;
 }
 

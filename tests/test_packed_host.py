@@ -130,6 +130,7 @@ CALL = dict(q=P, q_tok=1024, q_head=64, k=P, k_tok=1024, k_head=64, v=P, v_tok=1
     (dict(q=None), L.LBW_ERR_INVALID), (dict(v=None), L.LBW_ERR_INVALID), (dict(out=None), L.LBW_ERR_INVALID),
     (dict(cu_q=None), L.LBW_ERR_INVALID), (dict(dim=96), L.LBW_ERR_SHAPE), (dict(hk=3), L.LBW_ERR_SHAPE),
     (dict(hk=0), L.LBW_ERR_SHAPE), (dict(n=-1), L.LBW_ERR_SHAPE), (dict(tk=1 << 31), L.LBW_ERR_SHAPE),
+    (dict(tq=1 << 28), L.LBW_ERR_SHAPE), (dict(tq=1 << 62), L.LBW_ERR_SHAPE), (dict(n=1 << 30), L.LBW_ERR_SHAPE),
     (dict(dtype=2), L.LBW_ERR_INVALID), (dict(scale=0.0), L.LBW_ERR_INVALID), (dict(scale=math.nan), L.LBW_ERR_INVALID),
     (dict(scale=math.inf), L.LBW_ERR_INVALID), (dict(out_tok=1028), L.LBW_ERR_ALIGN),
     (dict(out=ctypes.c_void_p(4104)), L.LBW_ERR_ALIGN), (dict(cu_k=ctypes.c_void_p(4098)), L.LBW_ERR_ALIGN),
