@@ -760,7 +760,7 @@ def _device_index(who, *tensors):
 
 def _launch(dev, fn, *args):
     """fn(*args, the current stream of device dev) with dev as the current device (the library launches there)."""
-    if torch.cuda.current_device() == dev:
+    if torch._C._cuda_getDevice() == dev:   # (its tensors exist: CUDA is initialised)
         return fn(*args, raw_stream(dev))
     with torch.cuda.device(dev):
         return fn(*args, raw_stream(dev))
