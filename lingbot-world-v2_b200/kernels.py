@@ -766,45 +766,71 @@ def _launch(dev, fn, *args):
         return fn(*args, raw_stream(dev))
 
 
-def _rows3(who, name, t, dtype=None, dim=None, written=False):
+# Checks of shapes, strides and types, remembered by those values (lru_cache): a decoding loop passes the same ones in
+# every step, and checking them takes as long as the launch. What is checked by `form` is t.shape, t.stride(), t.dtype.
+
+def _form(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
+def _rows3(who, name, form, dtype=None, dim=None, written=False):
     """(tokens, heads, head_dim, token stride, head stride) of a [tokens, heads, head_dim] or [1, tokens, heads,
     head_dim] tensor with a contiguous head_dim."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3:
-        if len(shape) != 4 or shape[0] != 1:
-            raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(shape)}")
+    full, stride, own = form
+    shape = full
+    if len(shape) == 4 and shape[0] == 1:
         shape, stride = shape[1:], stride[1:]
-    tokens, heads, d = shape
-    tok, head, inner = stride
-    if heads < 1:
-        raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
-        raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
-    if dim is not None and d != dim:
-        raise ValueError(f"{who}: head_dim of {name} is {d}, expected {dim}")
-    if inner != 1 and d > 1:
+    if len(shape) != 3 or shape[1] < 1:
+        raise ValueError(f"{who}: {name} must be [tokens, heads, head_dim], got {tuple(full)}")
+    if dtype is not None and own != dtype:
+        raise ValueError(f"{who}: {name} is {own}, expected {dtype}")
+    if dim is not None and shape[2] != dim:
+        raise ValueError(f"{who}: head_dim of {name} is {shape[2]}, expected {dim}")
+    if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"{who}: {name} needs a contiguous head_dim")
-    if written and ((tok == 0 and tokens > 1) or (head == 0 and heads > 1)):
+    if written and ((stride[0] == 0 and shape[0] > 1) or (stride[1] == 0 and shape[1] > 1)):
         raise ValueError(f"{who}: {name} is an expanded tensor")
-    return tokens, heads, d, tok, head
+    return (*shape, stride[0], stride[1])
 
 
-def _positions(who, positions, tokens, rope):
-    """(pointer, bits, token stride, axis stride) of [tokens, axes] (or [tokens]) positions."""
-    shape, stride = positions.shape, positions.stride()
+def _positions(who, form, tokens, axes):
+    """(bits, token stride, axis stride) of [tokens, axes] (or [tokens]) positions."""
+    shape, stride, dtype = form
+    full = shape
     if len(shape) == 1:
         shape, stride = (shape[0], 1), (stride[0], 1)
-    if len(shape) != 2 or shape[0] != tokens or shape[1] != rope.axes:
-        raise ValueError(f"{who}: positions must be [{tokens}, {rope.axes}], got {tuple(positions.shape)}")
-    return positions.data_ptr(), _index_bits(who, "positions", positions), stride[0], stride[1]
+    if len(shape) != 2 or shape[0] != tokens or shape[1] != axes:
+        raise ValueError(f"{who}: positions must be [{tokens}, {axes}], got {tuple(full)}")
+    return _index_bits(who, "positions", dtype), stride[0], stride[1]
 
 
-def _index_bits(who, name, t):
-    if t.dtype == torch.int64:
+def _index_bits(who, name, dtype):
+    if dtype == torch.int64:
         return 64
-    if t.dtype != torch.int32:
-        raise ValueError(f"{who}: {name} must be int32 or int64, got {t.dtype}")
+    if dtype != torch.int32:
+        raise ValueError(f"{who}: {name} must be int32 or int64, got {dtype}")
     return 32
+
+
+def _vector(who, name, form, n, dtypes, kind):
+    """Check that a tensor is a contiguous vector of n values of one of the dtypes."""
+    shape, stride, dtype = form
+    if shape != (n,) or dtype not in dtypes or (n > 1 and stride[0] != 1):
+        raise ValueError(f"{who}: {name} must be contiguous {kind} [{n}], got {tuple(shape)} {dtype}")
+
+
+@functools.lru_cache(4096)
+def _axial_checks(x, out, positions, axes):
+    """(tokens, x token and head stride, out's, heads, head_dim, lbw_dtype, position bits and strides) of axial_rope."""
+    who, dtype = "axial_rope", x[2]
+    if dtype not in DTYPES:
+        raise ValueError(f"{who}: x is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
+    tokens, heads, dim, x_tok, x_head = _rows3(who, "x", x)
+    o_tokens, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
+    if o_tokens != tokens or o_heads != heads:
+        raise ValueError(f"{who}: out is {tuple(out[0])}, x {tuple(x[0])}")
+    return (tokens, x_tok, x_head, o_tok, o_head, heads, dim, DTYPES[dtype],
+            *_positions(who, positions, tokens, axes))
 
 
 def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
@@ -820,29 +846,52 @@ def axial_rope(x, positions, rope, inverse=False, out=None, _eager=False):
                  bool(inverse), out)
         return out
     dev = _device_index(who, x, positions, out)
-    dtype = x.dtype
-    if dtype not in DTYPES:
-        raise ValueError(f"{who}: x is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
-    tokens, heads, dim, x_tok, x_head = _rows3(who, "x", x)
     if out is None:
         out = torch.empty_like(x)
-    o_tokens, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
-    if o_tokens != tokens or o_heads != heads:
-        raise ValueError(f"{who}: out is {tuple(out.shape)}, x {tuple(x.shape)}")
-    pos = _positions(who, positions, tokens, rope)
+    tokens, x_tok, x_head, o_tok, o_head, heads, dim, dtype, bits, p_tok, p_axis = _axial_checks(
+        _form(x), _form(out), _form(positions), rope.axes)
     seg = HEAD_ROWS.pack(x.data_ptr(), out.data_ptr(), 0, x_tok, x_head, o_tok, o_head, heads, 0)
-    check(_launch(dev, load().lbw_axial_rope, seg, tokens, dim, DTYPES[dtype], *pos, rope.ref, 1 if inverse else 0), who,
-          launches=1 if tokens else 0)
+    check(_launch(dev, load().lbw_axial_rope, seg, tokens, dim, dtype, positions.data_ptr(), bits, p_tok, p_axis, rope.ref,
+                  1 if inverse else 0), who, launches=1 if tokens else 0)
     return out
 
 
-def _gain(who, name, g, dtype, dim):
-    """(pointer, is fp32) of a gain [dim]."""
-    if g is None:
-        return 0, 0
-    if g.shape != (dim,) or (g.dtype != dtype and g.dtype != torch.float32) or not g.is_contiguous():
-        raise ValueError(f"{who}: {name} must be contiguous [{dim}] {dtype} or fp32, got {tuple(g.shape)} {g.dtype}")
-    return g.data_ptr(), 1 if g.dtype == torch.float32 else 0
+@functools.lru_cache(4096)
+def _headnorm_checks(q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows, axes):
+    """What qk_headnorm_rope passes on: tokens, head_dim, lbw_dtype, the strides, heads and gain types of q, k and v,
+    position bits and strides, row bits, rows of the cache."""
+    who, dtype = "qk_headnorm_rope", q[2]
+    if dtype not in DTYPES:
+        raise ValueError(f"{who}: q is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
+    if (positions is None) != (axes is None):
+        raise ValueError(f"{who}: give positions and rope, or neither")
+    if (v is None) != (v_out is None) or (v is not None and k_rows is None):
+        raise ValueError(f"{who}: v is copied to the rows k_rows of v_out: give all three, or no v")
+    tokens, hq, dim, q_tok, q_head = _rows3(who, "q", q)
+    k_tokens, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
+    if k_tokens != tokens:
+        raise ValueError(f"{who}: {tokens} rows of q, {k_tokens} of k")
+    qo_rows, qo_heads, _, qo_row, qo_head = _rows3(who, "q_out", q_out, dtype, dim, written=True)
+    ko_rows, ko_heads, _, ko_row, ko_head = _rows3(who, "k_out", k_out, dtype, dim, written=True)
+    if qo_rows != tokens or qo_heads != hq or ko_heads != hk or (k_rows is None and ko_rows != tokens):
+        raise ValueError(f"{who}: q_out {tuple(q_out[0])} / k_out {tuple(k_out[0])} do not match q, k")
+    for name, g in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
+        if g is not None:
+            _vector(who, name, g, dim, (dtype, torch.float32), f"{dtype} or fp32")
+    wide = [1 if g is not None and g[2] == torch.float32 else 0 for g in (gamma_q, gamma_k)]
+    rows_bits, v_seg = 0, None
+    if k_rows is not None:
+        rows_bits = _index_bits(who, "k_rows", k_rows[2])
+        _vector(who, "k_rows", k_rows, tokens, (torch.int32, torch.int64), "int32 or int64")
+    if v is not None:
+        v_tokens, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
+        vo_rows, vo_heads, _, vo_row, vo_head = _rows3(who, "v_out", v_out, dtype, dim, written=True)
+        if v_tokens != tokens or vo_heads != hv or vo_rows != ko_rows:
+            raise ValueError(f"{who}: v {tuple(v[0])} / v_out {tuple(v_out[0])} do not match q and k_out")
+        v_seg = (v_tok, v_head, vo_row, vo_head, hv, 0)
+    pos = (32, 0, 0) if positions is None else _positions(who, positions, tokens, axes)
+    return (tokens, dim, DTYPES[dtype], (q_tok, q_head, qo_row, qo_head, hq, wide[0]),
+            (k_tok, k_head, ko_row, ko_head, hk, wide[1]), v_seg, pos, rows_bits, ko_rows)
 
 
 def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_out=None, k_out=None, v=None,
@@ -863,50 +912,20 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
                  k_rows)
         return q_out, k_out
     dev = _device_index(who, q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows)
-    dtype = q.dtype
-    if dtype not in DTYPES:
-        raise ValueError(f"{who}: q is {dtype}, expected one of {sorted(str(t) for t in DTYPES)}")
-    if (positions is None) != (rope is None):
-        raise ValueError(f"{who}: give positions and rope, or neither")
-    if (v is None) != (v_out is None) or (v is not None and k_rows is None):
-        raise ValueError(f"{who}: v is copied to the rows k_rows of v_out: give all three, or no v")
     if k_rows is not None and k_out is None:
         raise ValueError(f"{who}: k_rows name rows of k_out: give it")
-    tokens, hq, dim, q_tok, q_head = _rows3(who, "q", q)
-    k_tokens, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
-    if k_tokens != tokens:
-        raise ValueError(f"{who}: {tokens} rows of q, {k_tokens} of k")
     q_out = torch.empty_like(q) if q_out is None else q_out
     k_out = torch.empty_like(k) if k_out is None else k_out
-    qo_rows, qo_heads, _, qo_row, qo_head = _rows3(who, "q_out", q_out, dtype, dim, written=True)
-    ko_rows, ko_heads, _, ko_row, ko_head = _rows3(who, "k_out", k_out, dtype, dim, written=True)
-    if qo_rows != tokens or qo_heads != hq or ko_heads != hk or (k_rows is None and ko_rows != tokens):
-        raise ValueError(f"{who}: q_out {tuple(q_out.shape)} / k_out {tuple(k_out.shape)} do not match q, k")
-    gq, gq_f32 = _gain(who, "gamma_q", gamma_q, dtype, dim)
-    gk, gk_f32 = _gain(who, "gamma_k", gamma_k, dtype, dim)
-    seg_q = HEAD_ROWS.pack(q.data_ptr(), q_out.data_ptr(), gq, q_tok, q_head, qo_row, qo_head, hq, gq_f32)
-    seg_k = HEAD_ROWS.pack(k.data_ptr(), k_out.data_ptr(), gk, k_tok, k_head, ko_row, ko_head, hk, gk_f32)
-    seg_v, rows, rows_bits = None, None, 0
-    if k_rows is not None:
-        rows, rows_bits = k_rows.data_ptr(), _index_bits(who, "k_rows", k_rows)
-        if k_rows.shape != (tokens,) or not k_rows.is_contiguous():
-            raise ValueError(f"{who}: k_rows must be contiguous [{tokens}], got {tuple(k_rows.shape)}")
-    if v is not None:
-        v_tokens, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
-        vo_rows, vo_heads, _, vo_row, vo_head = _rows3(who, "v_out", v_out, dtype, dim, written=True)
-        if v_tokens != tokens or vo_heads != hv or vo_rows != ko_rows:
-            raise ValueError(f"{who}: v {tuple(v.shape)} / v_out {tuple(v_out.shape)} do not match q and k_out")
-        seg_v = HEAD_ROWS.pack(v.data_ptr(), v_out.data_ptr(), 0, v_tok, v_head, vo_row, vo_head, hv, 0)
-    pos = (None, 32, 0, 0) if rope is None else _positions(who, positions, tokens, rope)
-    check(_launch(dev, load().lbw_qk_headnorm_rope, seg_q, seg_k, seg_v, tokens, dim, DTYPES[dtype], eps, *pos,
-                  None if rope is None else rope.ref, rows, rows_bits, ko_rows), who, launches=1 if tokens else 0)
+    tokens, dim, dtype, of_q, of_k, of_v, pos, rows_bits, rows = _headnorm_checks(
+        _form(q), _form(k), _form(gamma_q), _form(gamma_k), _form(positions), _form(q_out), _form(k_out), _form(v),
+        _form(v_out), _form(k_rows), None if rope is None else rope.axes)
+    seg_q = HEAD_ROWS.pack(q.data_ptr(), q_out.data_ptr(), 0 if gamma_q is None else gamma_q.data_ptr(), *of_q)
+    seg_k = HEAD_ROWS.pack(k.data_ptr(), k_out.data_ptr(), 0 if gamma_k is None else gamma_k.data_ptr(), *of_k)
+    seg_v = None if of_v is None else HEAD_ROWS.pack(v.data_ptr(), v_out.data_ptr(), 0, *of_v)
+    check(_launch(dev, load().lbw_qk_headnorm_rope, seg_q, seg_k, seg_v, tokens, dim, dtype, eps,
+                  None if rope is None else positions.data_ptr(), *pos, None if rope is None else rope.ref,
+                  None if k_rows is None else k_rows.data_ptr(), rows_bits, rows), who, launches=1 if tokens else 0)
     return q_out, k_out
-
-
-def _int32(who, name, t, n):
-    """Check that t is a contiguous int32 vector of n values."""
-    if n < 0 or t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{who}: {name} must be contiguous int32 [{max(n, 0)}], got {tuple(t.shape)} {t.dtype}")
 
 
 @functools.lru_cache(4096)
@@ -918,6 +937,27 @@ def _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, same_lens, dev):
                                                     ctypes.byref(k)),
               "packed_attention_workspace")
     return b.value, k.value
+
+
+@functools.lru_cache(4096)
+def _packed_checks(q, k, v, out, cu_q, cu_k, k_lens):
+    """(tq, tk, hq, hk, head_dim, sequences, lbw_dtype, token and head strides of q, k, v and out) of packed_attention."""
+    who, dtype = "packed_attention", q[2]
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise ValueError(f"{who}: q is {dtype}, expected bf16 or fp16")
+    tq, hq, dim, q_tok, q_head = _rows3(who, "q", q)
+    tk, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
+    v_rows, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
+    if v_rows != tk or hv != hk:
+        raise ValueError(f"{who}: k {tuple(k[0])} and v {tuple(v[0])} differ")
+    n = cu_q[0][0] - 1 if len(cu_q[0]) == 1 else -1
+    for name, form, want in (("cu_q", cu_q, n + 1), ("cu_k", cu_k, n + 1), ("k_lens", k_lens, n)):
+        if form is not None:
+            _vector(who, name, form, max(want, 0), (torch.int32,), "int32")
+    o_rows, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
+    if o_rows != tq or o_heads != hq:
+        raise ValueError(f"{who}: out is {tuple(out[0])}, q {tuple(q[0])}")
+    return (tq, tk, hq, hk, dim, n, DTYPES[dtype], q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head)
 
 
 def packed_attention_workspace(tq, tk, hq, hk, head_dim, n_seqs, device, max_q=None, same_lens=False):
@@ -947,31 +987,16 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
         _op(who)(q, k, v, cu_q, cu_k, k_lens, bool(causal), float(scale), out, int(max_q or 0))
         return out
     dev = _device_index(who, q, k, v, cu_q, cu_k, k_lens, out, workspace)
-    dtype = q.dtype
-    if dtype != torch.bfloat16 and dtype != torch.float16:
-        raise ValueError(f"{who}: q is {dtype}, expected bf16 or fp16")
-    tq, hq, dim, q_tok, q_head = _rows3(who, "q", q)
-    tk, hk, _, k_tok, k_head = _rows3(who, "k", k, dtype, dim)
-    v_rows, hv, _, v_tok, v_head = _rows3(who, "v", v, dtype, dim)
-    if v_rows != tk or hv != hk:
-        raise ValueError(f"{who}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
-    _int32(who, "cu_q", cu_q, n + 1)
-    if cu_k is not cu_q:
-        _int32(who, "cu_k", cu_k, n + 1)
-    if k_lens is not None:
-        _int32(who, "k_lens", k_lens, n)
+    if out is None:
+        out = torch.empty_like(q)
+    tq, tk, hq, hk, dim, n, dtype, q_tok, q_head, k_tok, k_head, v_tok, v_head, o_tok, o_head = _packed_checks(
+        _form(q), _form(k), _form(v), _form(out), _form(cu_q), _form(cu_k), _form(k_lens))
     if max_q is None:
         max_q = 0
     elif max_q < 0:
         raise ValueError(f"{who}: max_q {max_q}")
     elif max_q > tq:
         max_q = tq
-    if out is None:
-        out = torch.empty_like(q)
-    o_rows, o_heads, _, o_tok, o_head = _rows3(who, "out", out, dtype, dim, written=True)
-    if o_rows != tq or o_heads != hq:
-        raise ValueError(f"{who}: out is {tuple(out.shape)}, q {tuple(q.shape)}")
     scale = 1.0 / math.sqrt(dim) if softmax_scale is None else float(softmax_scale)
     pq, pk = cu_q.data_ptr(), cu_k.data_ptr()
     ws_bytes, launches = _packed_attention_plan(tq, tk, hq, hk, dim, n, max_q, pq == pk and k_lens is None, dev)
@@ -983,7 +1008,7 @@ def packed_attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, softmax_scal
         workspace = q.new_empty(ws_bytes, dtype=torch.uint8)
     batch = PACKED_BATCH.pack(q.data_ptr(), q_tok, q_head, k.data_ptr(), k_tok, k_head, v.data_ptr(), v_tok, v_head,
                               out.data_ptr(), o_tok, o_head, pq, pk, 0 if k_lens is None else k_lens.data_ptr(), tq, tk,
-                              n, hq, hk, dim, DTYPES[dtype], 1 if causal else 0, max_q, scale)
+                              n, hq, hk, dim, dtype, 1 if causal else 0, max_q, scale)
     check(_launch(dev, load().lbw_packed_attention, batch, None if workspace is None else workspace.data_ptr(), ws_bytes),
           who, launches=launches)
     return out
