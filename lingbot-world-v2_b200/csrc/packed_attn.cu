@@ -908,7 +908,9 @@ static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, i
   const int group = hq / hk;
   const long long most = max_q > 0 && max_q < tq ? max_q : tq;
   p.tiles = most * group > SHORT_ROWS;
-  p.split = !p.tiles || (n_seqs > 1 && !same_lens);  // (as many keys as queries: a short sequence is one tile)
+  // Both kernels where there may be short sequences among the others: not where all have the promised number of rows, nor
+  // where they have as many keys as queries (a short one is one tile).
+  p.split = !p.tiles || (n_seqs > 1 && !same_lens && !(max_q > 0 && (long long)n_seqs * max_q == tq));
   p.split_rows = p.tiles ? SHORT_ROWS : LLONG_MAX;  // (a sequence longer than max_q promised is still computed)
   if (p.split) p.split_floats = split_workspace_floats(d);
   if (!p.tiles) return p;
@@ -920,9 +922,9 @@ static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, i
   long long pairs = tq / (2 * p.tile.tile_toks) + n_seqs;
   if (pairs > tq) pairs = tq;
   p.windows = pairs * p.tile.head_tiles;
-  const long long key_tiles = (tk + 127) / 128;
+  const long long key_tiles = n_seqs > 0 ? (tk / n_seqs + 127) / 128 : 0;
   // Few windows: their keys are cut into ranges while the windows fill the SMs at most once, each range of 4 key tiles or
-  // more, 16 ranges at most (a row's partial results are merged one after the other). Measured (us, with / without, 8
+  // more (of the mean sequence), 16 ranges at most (a row's partial results are merged one after the other). Measured (us, with / without, 8
   // heads): 200 queries of 30,000 keys 53 / 417, of 8,192 32 / 120, of 1,000 20 / 23; 1,000 of 8,192 50 / 121; 500 of 500
   // 15 / 15. Ranges of 2 tiles: 17 at 200 of 1,000, but 18 at 500 of 500; up to 64 ranges: 35 for 28 at 64 of 8,192; as
   // many as fill the SMs twice: 62 for 50 at 1,000 of 8,192.

@@ -371,6 +371,17 @@ def test_packed_attention_over_many_short_sequences(cuda_dev):
         assert po.within(x, want, bound) <= 1
 
 
+@pytest.mark.parametrize("q_lens", [[96, 96, 96], [1, 191, 96], [288, 0, 0], [2, 2, 284]])
+def test_packed_attention_where_max_q_says_all_are_alike(cuda_dev, q_lens):
+    """max_q times the sequences is the number of rows: true or not, every row is computed."""
+    import lbw_b200.kernels as K
+    for k_lens in ([550, 110, 429], [300, 200, 300]):
+        q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, 8, 2, 128, BF)
+        ws = K.packed_attention_workspace(288, sum(k_lens), 8, 2, 128, 3, cuda_dev, max_q=96)
+        want, bound = po.attention(q, k, v, cu_q, cu_k)
+        assert po.within(K.packed_attention(q, k, v, cu_q, cu_k, max_q=96, workspace=ws), want, bound) <= 1
+
+
 @pytest.mark.parametrize("heads,q_lens,k_lens", [((4, 4), [200], [3000]), ((8, 1), [2], [9000]), ((8, 2), [1] * 3, [5000, 64, 1])])
 def test_packed_attention_in_place_where_keys_are_split(cuda_dev, heads, q_lens, k_lens):
     """Blocks that share a query's keys all read it before any of them writes its row."""
