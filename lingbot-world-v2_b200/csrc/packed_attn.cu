@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
             const int all_p = (keys_p + BN - 1) / BN, all_s = (keys_s + BN - 1) / BN;
             w.g0 = 0;
             w.n_p = all_p;
-            if (ta.n_split > 1) {  // (n_split <= 16 and all_p < 2^24: no overflow)
+            if (ta.n_split > 1) {  // (n_split <= 32 and all_p < 2^24: no overflow)
               w.g0 = w.split * all_p / ta.n_split;
               w.n_p = (w.split + 1) * all_p / ta.n_split - w.g0;
             }
@@ -818,19 +818,39 @@ __global__ void __launch_bounds__(128) packed_merge_kernel(const __grid_constant
   }
   pdl_wait();
   if (!__any_sync(0xffffffffu, ours)) return;
+  // Lane z weighs range z (at most 32); then the rows, with the loads of 8 ranges in flight.
   const long long step = (long long)a.tq * a.hq;
-  float M = -INFINITY;
-  for (int z = 0; z < ta.n_split; ++z) M = fmaxf(M, ta.part_ml[(z * step + wid) * 2]);
-  constexpr int PER = D / 32;
-  float L = 0.f, acc[PER] = {};
-  for (int z = 0; z < ta.n_split; ++z) {
-    const float2 ml = *reinterpret_cast<const float2*>(ta.part_ml + (z * step + wid) * 2);
-    if (ml.y == 0.f) continue;  // no key of this range is visible: nothing was written
-    const float w = ml.x == -INFINITY ? ml.y : exp2f(ml.x - M);  // (all scores NaN: so is the sum)
-    L += w * ml.y;
-    const float* o = ta.part_o + (z * step + wid) * D + lane * PER;
+  const float2 ml = lane < ta.n_split ? *reinterpret_cast<const float2*>(ta.part_ml + (lane * step + wid) * 2)
+                                      : make_float2(-INFINITY, 0.f);
+  float M = ml.x;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] += w * o[i];
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const bool some = ml.y != 0.f;  // (no key of the range visible: nothing was written. All scores NaN: so is the sum)
+  const float w = !some ? 0.f : ml.x == -INFINITY ? ml.y : exp2f(ml.x - M);
+  float L = some ? w * ml.y : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  constexpr int PER = D / 32, UN = 8;
+  const uint32_t there = __ballot_sync(0xffffffffu, some);
+  float acc[PER] = {};
+  for (int z = 0; z < ta.n_split; z += UN) {
+    float f[UN][PER];
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const float* o = ta.part_o + ((z + i) * step + wid) * D + lane * PER;
+#pragma unroll
+      for (int e = 0; e < PER; e += 2) {
+        const float2 v = there >> (z + i) & 1 ? *reinterpret_cast<const float2*>(o + e) : make_float2(0.f, 0.f);
+        f[i][e] = v.x;
+        f[i][e + 1] = v.y;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const float wz = __shfl_sync(0xffffffffu, w, z + i);
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] += wz * f[i][e];
+    }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + tok * a.os_tok + head * a.os_head +
@@ -922,15 +942,20 @@ static PackedPlan make_plan(long long tq, long long tk, int hq, int hk, int d, i
   long long pairs = tq / (2 * p.tile.tile_toks) + n_seqs;
   if (pairs > tq) pairs = tq;
   p.windows = pairs * p.tile.head_tiles;
+  // Few windows: their keys are cut into ranges while the windows fill the SMs at most once, from 8 key tiles (of the mean
+  // sequence) on, 16 for two ranges, each of 2 tiles or more, and of 8 or more beyond 16 ranges; 32 at most (a lane each in
+  // the merge).
+  // Measured (us, with / without, 8 heads): 200 queries of 30,000 keys 44 / 417, of 8,192 25 / 120, of 1,000 16 / 23; 1,000
+  // of 8,192 48 / 121. Ranges of 4 tiles at least: 20 at 200 of 1,000, 18 for 15 at 128 of 4,096; ranges from 4 tiles on: 17
+  // for 15 at 500 of 500, 24 for 18 at 3 x 96 of 550; 16 ranges at most: 68 for 44 at 64 of 60,000; 32 of any length: 26.6
+  // for 24.9 at 40 of 16,000; as many as fill the SMs twice: 62 for 50 at 1,000 of 8,192. Two ranges / one, 32 heads over 8:
+  // 26.8 / 24.5 at 3 x 96 of 1,000, 33.8 / 38.4 of 2,000; 35.8 / 30.3 at 1,500 of 1,500 (12 heads).
   const long long key_tiles = n_seqs > 0 ? (tk / n_seqs + 127) / 128 : 0;
-  // Few windows: their keys are cut into ranges while the windows fill the SMs at most once, each range of 4 key tiles or
-  // more (of the mean sequence), 16 ranges at most (a row's partial results are merged one after the other). Measured (us, with / without, 8
-  // heads): 200 queries of 30,000 keys 53 / 417, of 8,192 32 / 120, of 1,000 20 / 23; 1,000 of 8,192 50 / 121; 500 of 500
-  // 15 / 15. Ranges of 2 tiles: 17 at 200 of 1,000, but 18 at 500 of 500; up to 64 ranges: 35 for 28 at 64 of 8,192; as
-  // many as fill the SMs twice: 62 for 50 at 1,000 of 8,192.
   long long split = p.windows > 0 ? num_sms() / p.windows : 1;
-  if (split > key_tiles / 4) split = key_tiles / 4;
-  if (split > 16) split = 16;
+  if (split > key_tiles / 2) split = key_tiles / 2;
+  if (split > 16 && split > key_tiles / 8) split = key_tiles / 8 > 16 ? key_tiles / 8 : 16;
+  if (split > 32) split = 32;
+  if (key_tiles < (split == 2 ? 16 : 8)) split = 1;
   p.tile.n_split = split < 1 ? 1 : (int)split;
   if (p.tile.n_split > 1) p.tile_floats = (long long)p.tile.n_split * tq * hq * (d + 2);
   return p;
@@ -978,7 +1003,7 @@ int lbw_packed_attention(const lbw_packed_batch* batch, void* workspace, long lo
   if (!aligned(cu_q, 4) || !aligned(cu_k, 4) || !aligned(k_lens, 4) || !aligned(out, 16) || out_tok % 8 || out_head % 8)
     return set_error(LBW_ERR_ALIGN, "%s: the output needs a 16-byte aligned pointer and strides", who);
   const PackedPlan p = make_plan(tq, tk, hq, hk, head_dim, n_seqs, max_q, cu_q == cu_k && !k_lens);
-  if (p.windows * 16 >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
+  if (p.windows * 32 >= 1ll << 31) return set_error(LBW_ERR_SHAPE, "%s: %lld windows", who, p.windows);
   const long long need = (p.tile_floats + p.split_floats) * 4;
   if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
     return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who, need,

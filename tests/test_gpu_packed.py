@@ -382,6 +382,20 @@ def test_packed_attention_where_max_q_says_all_are_alike(cuda_dev, q_lens):
         assert po.within(K.packed_attention(q, k, v, cu_q, cu_k, max_q=96, workspace=ws), want, bound) <= 1
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,q_lens,k_lens", [(64, [40], [40000]), (128, [20, 33], [20000, 25000]), (128, [25], [2049])])
+def test_packed_attention_in_up_to_32_key_ranges(cuda_dev, dim, q_lens, k_lens, causal):
+    """Few rows over many keys: 32 ranges, ranges of two sequences, ranges of two tiles; one range all NaN in its keys."""
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, q_lens, k_lens, 2, 1, dim, BF, qk_scale=0.5)
+    want, bound = po.attention(q, k, v, cu_q, cu_k, causal=causal)
+    assert po.within(K.packed_attention(q, k, v, cu_q, cu_k, causal=causal), want, bound) <= 1
+    k[300:1800] = float("nan")
+    out = K.packed_attention(q, k, v, cu_q, cu_k, causal=causal)
+    assert torch.isnan(out[:q_lens[0]].float()).all()
+    assert po.within(out[q_lens[0]:], want[q_lens[0]:], bound[q_lens[0]:]) <= 1
+
+
 @pytest.mark.parametrize("heads,q_lens,k_lens", [((4, 4), [200], [3000]), ((8, 1), [2], [9000]), ((8, 2), [1] * 3, [5000, 64, 1])])
 def test_packed_attention_in_place_where_keys_are_split(cuda_dev, heads, q_lens, k_lens):
     """Blocks that share a query's keys all read it before any of them writes its row."""
