@@ -909,8 +909,8 @@ static int pick_pack(int group, long long avg) {
 
 // Rows per kv head (queries x group) up to which a sequence is packed_split_kernel's, which has 16 in a unit: it reads the
 // keys and values once for each unit, the tile kernel once for 256 rows. Measured (us, split / tile kernel, 8 kv heads,
-// 128 wide) at 1, 16 and 32 rows: 32 x 16,384 keys 326 / 417, 336 / 425, 655 / 425; 8 x 4,096 31 / 40, 33 / 37, 45 / 37;
-// 1 x 30,000 28 / 40, 31 / 40, 50 / 41; 1 x 1,000 8 / 14, 10 / 14, 12 / 15; 128 x 500 50 / 65, 59 / 67, 133 / 66.
+// 128 wide) at 1, 16 and 32 rows: 32 x 16,384 keys 329 / 422, 341 / 431, 655 / 430; 8 x 4,096 33 / 42, 35 / 39, 42 / 37;
+// 1 x 30,000 28 / 34, 31 / 37, 48 / 37; 1 x 1,000 8 / 11, 10 / 11, 11 / 11; 128 x 500 50 / 67, 61 / 71, 108 / 68.
 constexpr int SHORT_ROWS = 16;
 
 // The call's launch plan, from the host's numbers alone. The sequences' own lengths are on the device: where they may be

@@ -13,7 +13,7 @@
 // rate (a warp spends ~150 instructions on 16 keys = 8 KB; the SM's share of the memory rate is 23 bytes a clock).
 // Bound: the bytes of K and V. Measured (B200, bf16, 128-wide heads, 8 kv heads, both kernels, replayed from a graph):
 // 32 sequences of 16,384 keys 326 us with 1 row per kv head, 336 with 16 (6.6 and 6.4 TB/s: a plain copy's rate);
-// 128 x 500 keys 50 and 59 us (5.3 and 4.4 TB/s: 7 units a CTA, whose ends - the join of 8 warps, masks, the next Q - are
+// 128 x 500 keys 50 and 60 us (5.3 and 4.4 TB/s: 7 units a CTA, whose ends - the join of 8 warps, masks, the next Q - are
 // not all hidden behind 8 tiles of loads); 1 x 30,000 keys 28 and 31 us (4.3 and 4.0 TB/s); 1 x 1,000 keys 8.2 and 10.4 us,
 // which is two launches, the look-up of the sequences and one trip to memory.
 #include "host_common.cuh"
