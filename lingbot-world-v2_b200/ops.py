@@ -294,3 +294,24 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
 @packed_attention.register_fake
 def _(q, k, v, cu_q, cu_k, k_lens, causal, scale, out, max_q):
     return None
+
+
+# These operators write into tensors that they are given, for which torch.library can hold no gradient formula: without
+# one a call that needs a gradient would go through and leave its outputs without any. The eager calls refuse it, and so
+# do the operators' entries for tensors that autograd watches, called directly or by a graph that is being traced.
+_LIB = torch.library.Library("lbw", "IMPL")
+
+
+def _refuse_gradients(name):
+    def entry(*args, **kwargs):
+        if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                           for t in (*args, *kwargs.values())):
+            raise ValueError(f"{name} has no gradient: call it under torch.no_grad() or with detached tensors")
+        with torch._C._AutoDispatchBelowAutograd():
+            return getattr(torch.ops.lbw, name).default(*args, **kwargs)
+
+    _LIB.impl(name, entry, "Autograd", allow_override=True)
+
+
+for _name in ("axial_rope", "qk_headnorm_rope", "packed_attention"):
+    _refuse_gradients(_name)
