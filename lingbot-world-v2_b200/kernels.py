@@ -903,6 +903,8 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
     [rows, hk, head_dim], and v, copied, to the same rows of v_out; tokens whose row lies outside the cache (-1: padding)
     write none. q_out may be q and, without k_rows, k_out may be k."""
     who = "qk_headnorm_rope"
+    if k_rows is not None and k_out is None:
+        raise ValueError(f"{who}: k_rows name rows of k_out: give it")
     if _tracing(_eager):
         q_out = torch.empty_like(q) if q_out is None else q_out
         k_out = torch.empty_like(k) if k_out is None else k_out
@@ -912,8 +914,6 @@ def qk_headnorm_rope(q, k, gamma_q, gamma_k, eps, positions=None, rope=None, q_o
                  k_rows)
         return q_out, k_out
     dev = _device_index(who, q, k, gamma_q, gamma_k, positions, q_out, k_out, v, v_out, k_rows)
-    if k_rows is not None and k_out is None:
-        raise ValueError(f"{who}: k_rows name rows of k_out: give it")
     q_out = torch.empty_like(q) if q_out is None else q_out
     k_out = torch.empty_like(k) if k_out is None else k_out
     tokens, dim, dtype, of_q, of_k, of_v, pos, rows_bits, rows = _headnorm_checks(

@@ -54,3 +54,18 @@ def test_compiled_graph_refuses_a_gradient(call, fullgraph):
     f = torch.compile(call, fullgraph=fullgraph, backend="aot_eager")
     with pytest.raises(Exception, match="has no gradient"):
         f(_x(True), GAIN.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("fullgraph", [True, False])
+def test_compiled_graph_refuses_cache_rows_without_a_cache(fullgraph):
+    """k_rows name rows of k_out: without it there is no cache that they could be rows of."""
+    rows = torch.arange(4)
+
+    def call(x):
+        return K.qk_headnorm_rope(x, x, None, None, 1e-6, POS, ROPE, k_rows=rows)[1]
+
+    with pytest.raises(ValueError, match="k_rows name rows of k_out"):
+        call(_x())
+    torch._dynamo.reset()
+    with pytest.raises(Exception, match="k_rows name rows of k_out"):
+        torch.compile(call, fullgraph=fullgraph, backend="aot_eager")(_x())
