@@ -243,11 +243,14 @@ enum lbw_rope_layout {
   LBW_ROPE_HALF = 1         /* pair i = dims (i, i + pairs) */
 };
 /* A rotation of `pairs` pairs (a multiple of 4, at most 128): pair i turns by position `axis[i]` times f_i, given as
- * step[i] = round(f_i / (2 pi) * 2^64) mod 2^64, so that position * step wraps exactly at whole turns. */
+ * step[i] = floor(f_i / (2 pi) * 2^64) mod 2^64, so that position * step wraps exactly at whole turns: off by less than
+ * |position| * 2^-64 turns. wide != 0: the next 64 bits follow in step_low[i] (used for 64-bit positions), and no position
+ * loses anything that fp32 shows; wide = 0: step_low is not read. */
 typedef struct {
-  int pairs, axes, layout, reserved;
+  int pairs, axes, layout, wide;
   unsigned char axis[128];
   unsigned long long step[128];
+  unsigned long long step_low[128];
 } lbw_rope_axes;
 /* An operand of the row kernels: x [tokens, heads, head_dim] -> out [rows, heads, head_dim]; gamma [head_dim] of the
  * tensors' type (or fp32 with gamma_f32), or NULL for no gain. */

@@ -5,9 +5,11 @@
 //   n_d  = x_d * rsqrt(mean_d(x_d^2) + eps) * gamma_d            (norm form; n = x otherwise)
 //   t_i  = pos[axis(i)] * f_i                                    (angle of pair i)
 //   y    = (a cos t - b sin t, a sin t + b cos t)                for the pair (a, b) of n; dims beyond 2R: y = n
-// All in fp32 with one rounding to the output type. The angle is reduced exactly: with F_i = round(f_i / 2pi * 2^64)
-// the integer product pos * F_i mod 2^64 IS the angle in 2^-64 turns, for any 64-bit position of either sign, so far
-// positions lose nothing (an fp32 product pos * f_i is 6e-3 rad off at position 100,000).
+// All in fp32 with one rounding to the output type. The angle is reduced in integers: with F_i = floor(f_i / 2pi * 2^64)
+// the product pos * F_i mod 2^64 is the angle in 2^-64 turns, off by less than |pos| of them: below 2^-32 turns for every
+// 32-bit position, where the 24 bits that sincospif takes are off by 2^-26 (an fp32 product pos * f_i is 6e-3 rad off at
+// position 100,000). 64-bit positions take 64 more bits of f_i / 2pi, F' : the upper half of pos * (F_i 2^64 + F'_i) mod
+// 2^128 is off by less than 2^-63 turns at any of them (F_i alone: 4e-7 rad at 2^40, 4e-4 at 2^50, nothing right at 2^63).
 //
 // Bound: bytes (each value read once and written once, ~7 flops each). A head is D / 8 "units" of 8 values, one per
 // lane: unit u holds the pairs 4u .. 4u + 3, which are 8 neighbouring values (interleaved pairs: one 16-byte access)
@@ -17,6 +19,9 @@
 // Measured (B200, 10,800 tokens, 128-wide heads, bf16): norm of 40 + 40 heads out of the fused projection 78 us (442 MB,
 // 5.7 TB/s, 87% of a plain copy's rate; 84 us in the half layout), rotation of 120 heads 109-114 us (5.8-6.1 TB/s).
 #include <cuda_fp16.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "host_common.cuh"
 #include "lbw_common.cuh"
@@ -51,7 +56,17 @@ struct HeadArgs {
   const void* rows;
   int rows_bits;
   long long out_rows;
-  lbw_rope_axes rope;
+  struct {  // the part of lbw_rope_axes that every call needs
+    int pairs, layout;
+    unsigned char axis[128];
+    unsigned long long step[128];
+  } rope;
+};
+
+// A call with 64-bit positions and 128-bit steps has kernels of its own: with the lower halves in all, calls with 32-bit
+// positions took 0.5 us more on the host (1 KB of arguments) and the kernel 0.7 to 1.2%.
+struct HeadArgsWide : HeadArgs {
+  unsigned long long step_low[128];
 };
 
 template <typename T>
@@ -229,13 +244,15 @@ LBW_DEV void head_copy(const HeadSeg& g, long long tok, long long row, bool on, 
 
 // Work item = (32 / G neighbouring tokens, chunk of the q | k | v heads), one warp each, grid-stride; a group of G lanes
 // has one token.
-template <typename T, bool NORM, bool HALF, int G>
-__global__ void __launch_bounds__(hr::THREADS, hr::MINB) head_rope_kernel(const __grid_constant__ HeadArgs a) {
-  __shared__ __align__(16) unsigned long long step[128];
+template <typename T, bool NORM, bool HALF, int G, typename A>
+__global__ void __launch_bounds__(hr::THREADS, hr::MINB) head_rope_kernel(const __grid_constant__ A a) {
+  constexpr bool WIDE = std::is_same_v<A, HeadArgsWide>;
+  __shared__ __align__(16) unsigned long long step[128], step_low[WIDE ? 128 : 1];
   __shared__ __align__(4) unsigned char axis[128];
   for (int i = threadIdx.x; i < a.rope.pairs; i += hr::THREADS) {
     step[i] = a.rope.step[i];
     axis[i] = a.rope.axis[i];
+    if constexpr (WIDE) step_low[i] = a.step_low[i];
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -260,7 +277,11 @@ __global__ void __launch_bounds__(hr::THREADS, hr::MINB) head_rope_kernel(const 
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
         const long long ps = load_index(a.pos, a.pos_bits, tok * a.ps_tok + axs[p] * a.ps_axis);
-        const unsigned long long turns = (unsigned long long)ps * step[4 * u + p];
+        unsigned long long turns = (unsigned long long)ps * step[4 * u + p];
+        if constexpr (WIDE) {  // the carry of the lower halves; a negative position is ps + 2^64 as an unsigned factor
+          const unsigned long long low = step_low[4 * u + p];
+          turns += __umul64hi((unsigned long long)ps, low) - (ps < 0 ? low : 0ull);
+        }
         sincospif((float)(int)(turns >> 32) * 4.656612873077393e-10f, &s[p], &c[p]);  // 2^-31: half turns in [-1, 1]
       }
     }
@@ -321,26 +342,42 @@ static int check_common(const char* who, long long tokens, int head_dim, int dty
   return LBW_OK;
 }
 
-template <typename T, bool NORM, bool HALF>
-static void launch_g(const HeadArgs& a, int group, unsigned blocks, cudaStream_t s) {
+// The rotation of the call, turned the other way if `inverse`; of a description without the lower halves only what it has
+// is read.
+static void set_rope(HeadArgsWide& a, bool& wide, const lbw_rope_axes& rope, bool inverse) {
+  wide = rope.wide && a.pos_bits == 64;
+  a.rope.pairs = rope.pairs;
+  a.rope.layout = rope.layout;
+  memcpy(a.rope.axis, rope.axis, rope.pairs);
+  memcpy(a.rope.step, rope.step, rope.pairs * 8);
+  if (wide) memcpy(a.step_low, rope.step_low, rope.pairs * 8);
+  for (int i = 0; inverse && i < rope.pairs; ++i) {  // minus the 64- or 128-bit number
+    a.rope.step[i] = ~a.rope.step[i] + (!wide || a.step_low[i] == 0);
+    if (wide) a.step_low[i] = 0ull - a.step_low[i];
+  }
+}
+
+template <typename T, bool NORM, bool HALF, typename A>
+static void launch_g(const A& a, int group, unsigned blocks, cudaStream_t s) {
   if (group == 8)
-    head_rope_kernel<T, NORM, HALF, 8><<<blocks, hr::THREADS, 0, s>>>(a);
+    head_rope_kernel<T, NORM, HALF, 8, A><<<blocks, hr::THREADS, 0, s>>>(a);
   else if (group == 16)
-    head_rope_kernel<T, NORM, HALF, 16><<<blocks, hr::THREADS, 0, s>>>(a);
+    head_rope_kernel<T, NORM, HALF, 16, A><<<blocks, hr::THREADS, 0, s>>>(a);
   else
-    head_rope_kernel<T, NORM, HALF, 32><<<blocks, hr::THREADS, 0, s>>>(a);
+    head_rope_kernel<T, NORM, HALF, 32, A><<<blocks, hr::THREADS, 0, s>>>(a);
 }
 
 template <typename T, bool NORM>
-static void launch_t(const HeadArgs& a, int group, unsigned blocks, cudaStream_t s) {
+static void launch_t(const HeadArgsWide& a, bool wide, int group, unsigned blocks, cudaStream_t s) {
+  const HeadArgs& narrow = a;
   if (a.rope.layout == LBW_ROPE_HALF)
-    launch_g<T, NORM, true>(a, group, blocks, s);
+    wide ? launch_g<T, NORM, true>(a, group, blocks, s) : launch_g<T, NORM, true>(narrow, group, blocks, s);
   else
-    launch_g<T, NORM, false>(a, group, blocks, s);
+    wide ? launch_g<T, NORM, false>(a, group, blocks, s) : launch_g<T, NORM, false>(narrow, group, blocks, s);
 }
 
 template <bool NORM>
-static int launch_head_rope(HeadArgs& a, int dtype, cudaStream_t s, const char* who) {
+static int launch_head_rope(HeadArgsWide& a, bool wide, int dtype, cudaStream_t s, const char* who) {
   a.units = a.dim / 8;
   const int group = a.units <= 8 ? 8 : a.units <= 16 ? 16 : 32;
   const int total = a.seg[0].heads + a.seg[1].heads + a.seg[2].heads;
@@ -364,11 +401,11 @@ static int launch_head_rope(HeadArgs& a, int dtype, cudaStream_t s, const char* 
   const long long want = (items + hr::THREADS / 32 - 1) / (hr::THREADS / 32);
   const unsigned blocks = (unsigned)(want < most ? want : most);
   if (dtype == LBW_BF16)
-    launch_t<__nv_bfloat16, NORM>(a, group, blocks, s);
+    launch_t<__nv_bfloat16, NORM>(a, wide, group, blocks, s);
   else if (dtype == LBW_FP16)
-    launch_t<__half, NORM>(a, group, blocks, s);
+    launch_t<__half, NORM>(a, wide, group, blocks, s);
   else
-    launch_t<float, NORM>(a, group, blocks, s);
+    launch_t<float, NORM>(a, wide, group, blocks, s);
   return cuda_check(cudaGetLastError(), who);
 }
 
@@ -382,7 +419,8 @@ int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int d
   if (err) return err;
   if (tokens == 0) return LBW_OK;
   if ((err = check_seg(who, "x", *x, dtype))) return err;
-  HeadArgs a{};
+  HeadArgsWide a;
+  static_cast<HeadArgs&>(a) = HeadArgs{};
   a.seg[0] = HeadSeg{x->x, x->out, nullptr, x->x_tok, x->x_head, x->out_row, x->out_head, x->heads, 0};
   if ((err = check_in_place(who, a.seg[0], tokens, false))) return err;
   a.tokens = tokens;
@@ -391,10 +429,9 @@ int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int d
   a.pos_bits = pos_bits;
   a.ps_tok = pos_tok;
   a.ps_axis = pos_axis;
-  a.rope = *rope;
-  if (inverse)
-    for (int i = 0; i < a.rope.pairs; ++i) a.rope.step[i] = 0ull - a.rope.step[i];
-  return launch_head_rope<false>(a, dtype, reinterpret_cast<cudaStream_t>(stream), "axial_rope launch");
+  bool wide;
+  set_rope(a, wide, *rope, inverse != 0);
+  return launch_head_rope<false>(a, wide, dtype, reinterpret_cast<cudaStream_t>(stream), "axial_rope launch");
 }
 
 int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
@@ -410,7 +447,8 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
     return set_error(LBW_ERR_INVALID, "%s: %d-bit cache rows", who, k_rows_bits);
   if (tokens == 0) return LBW_OK;
   if (k_rows && out_rows < 0) return set_error(LBW_ERR_SHAPE, "%s: %lld cache rows", who, out_rows);
-  HeadArgs a{};
+  HeadArgsWide a;
+  static_cast<HeadArgs&>(a) = HeadArgs{};
   const lbw_head_rows* in[3] = {q, k, v};
   const char* names[3] = {"q", "k", "v"};
   for (int i = 0; i < 3; ++i) {
@@ -433,8 +471,9 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
   a.rows = k_rows;
   a.rows_bits = k_rows_bits;
   a.out_rows = out_rows;
-  if (rope) a.rope = *rope;
-  return launch_head_rope<true>(a, dtype, reinterpret_cast<cudaStream_t>(stream), "qk_headnorm_rope launch");
+  bool wide = false;
+  if (rope) set_rope(a, wide, *rope, false);
+  return launch_head_rope<true>(a, wide, dtype, reinterpret_cast<cudaStream_t>(stream), "qk_headnorm_rope launch");
 }
 
 }  // extern "C"

@@ -10,6 +10,7 @@ are taken on the CPU in fp32 exactly as the reference does, so the tables are bi
 reference grids' entries.
 """
 import ctypes
+import decimal
 import math
 
 import torch
@@ -83,8 +84,35 @@ def _tables(freqs, f, h, w, start_frame, device):
 
 class RopeAxes(ctypes.Structure):
     """lbw_rope_axes (include/lbw.h)."""
-    _fields_ = [("pairs", ctypes.c_int), ("axes", ctypes.c_int), ("layout", ctypes.c_int), ("reserved", ctypes.c_int),
-                ("axis", ctypes.c_ubyte * 128), ("step", ctypes.c_ulonglong * 128)]
+    _fields_ = [("pairs", ctypes.c_int), ("axes", ctypes.c_int), ("layout", ctypes.c_int), ("wide", ctypes.c_int),
+                ("axis", ctypes.c_ubyte * 128), ("step", ctypes.c_ulonglong * 128), ("step_low", ctypes.c_ulonglong * 128)]
+
+
+def _pi(digits):
+    """pi to `digits` decimal digits: 16 atan(1/5) - 4 atan(1/239) (Machin's formula) in integers."""
+    one = 10 ** (digits + 10)
+
+    def atan(n):
+        total, term, k = 0, one // n, 1
+        while term:
+            total += term // k if k % 4 == 1 else -(term // k)
+            term //= n * n
+            k += 2
+        return total
+
+    return decimal.Decimal(16 * atan(5) - 4 * atan(239)) / one
+
+
+def _frequency(theta, exponent, scale):
+    """f = scale * theta^-exponent, exponent a pair (numerator, denominator), as a float, and the turns that it makes per
+    position, round(f / (2 pi) * 2^128) mod 2^128. (From the float, with its 53 bits, an angle is 0.07 rad off at position
+    2^50.)"""
+    with decimal.localcontext() as c:
+        size = abs(math.log10(theta)) + (abs(math.log10(abs(scale))) if scale else 0)
+        c.prec = 60 + int(size)   # 2^128 has 39 digits
+        c.rounding = decimal.ROUND_HALF_EVEN
+        f = decimal.Decimal(scale) * decimal.Decimal(theta) ** (decimal.Decimal(-exponent[0]) / exponent[1])
+        return float(f), int((f * 2 ** 127 / _pi(c.prec)).to_integral_value()) % (1 << 128)
 
 
 class AxialRope:
@@ -122,15 +150,15 @@ class AxialRope:
         if not (math.isfinite(self.theta) and self.theta > 0):
             raise ValueError(f"AxialRope: theta {theta!r}")
         self.axis_of_pair = [a for a, n in enumerate(self.sections) for _ in range(n)]
-        self.inv_freq = []                                   # radians per position, 64 bits
+        self.inv_freq = []                                   # radians per position, as floats
+        self.c = RopeAxes(self.pairs, self.axes, self.LAYOUTS[layout], 1)
         for a, n in enumerate(self.sections):
             for j in range(n):
-                e = j / n if spectrum == "axis" else len(self.inv_freq) / self.pairs
-                self.inv_freq.append(self.scale[a] * self.theta ** -e)
-        self.c = RopeAxes(self.pairs, self.axes, self.LAYOUTS[layout], 0)
-        for i, f in enumerate(self.inv_freq):
-            self.c.axis[i] = self.axis_of_pair[i]
-            self.c.step[i] = round(f / (2 * math.pi) * 2.0 ** 64) % (1 << 64)
+                i = len(self.inv_freq)
+                f, turns = _frequency(self.theta, (j, n) if spectrum == "axis" else (i, self.pairs), self.scale[a])
+                self.inv_freq.append(f)
+                self.c.axis[i] = a
+                self.c.step[i], self.c.step_low[i] = turns >> 64, turns & (1 << 64) - 1
         self.ref = ctypes.byref(self.c)
 
     def __reduce__(self):

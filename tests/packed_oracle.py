@@ -2,6 +2,8 @@
 
 The bounds count roundings. u = eps / 2 of the tensors' type is half a step (bf16 2^-8, fp16 2^-11, fp32 2^-24).
 """
+import decimal
+import functools
 import math
 
 import torch
@@ -57,19 +59,41 @@ def attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, scale=None):
     return out, bound
 
 
+TURN = 192   # bits of a turn in `turns_per_position`
+
+
+@functools.lru_cache(None)
+def turns_per_position(sections, theta, spectrum, scale):
+    """round(scale theta^-e / (2 pi) 2^192) of every pair, from the description alone: exp and ln with 150 digits, pi by the
+    arithmetic-geometric mean."""
+    D = decimal.Decimal
+    with decimal.localcontext() as c:
+        c.prec = 150
+        a, b, t, p = D(1), 1 / D(2).sqrt(), D(1) / 4, D(1)
+        for _ in range(9):
+            a, b, t, p = (a + b) / 2, (a * b).sqrt(), t - p * ((a - b) / 2) ** 2, 2 * p
+        pi = (a + b) ** 2 / (4 * t)
+        out, pairs = [], sum(sections)
+        for axis, n in enumerate(sections):
+            for j in range(n):
+                e = D(j) / n if spectrum == "axis" else D(len(out)) / pairs
+                f = D(scale[axis]) * (-e * D(theta).ln()).exp()
+                out.append(int((f / (2 * pi) * 2 ** TURN).to_integral_value()))
+    return out
+
+
 def rotate(x, positions, rope, inverse=False):
-    """(y, size) fp64: x [tokens, heads, d] fp64 rotated by rope at integer positions, and |a| + |b| of each pair."""
-    turns = torch.tensor(rope.inv_freq, dtype=torch.float64)
+    """(y, size) fp64: x [tokens, heads, d] fp64 rotated by rope at integer positions, and |a| + |b| of each pair. The
+    position times the turns per position is an integer, reduced exactly (fp64 loses digits beyond position 2^20)."""
     pos = positions.cpu()
     pos = pos[:, None] if pos.dim() == 1 else pos
-    # positions beyond 2^20 make the fp64 product lose digits: reduce the position times the frequency in integers
-    step = [round(f / (2 * math.pi) * 2 ** 64) for f in rope.inv_freq]
-    assert len(step) == len(turns)
+    step = turns_per_position(rope.sections, rope.theta, rope.spectrum, rope.scale)
+    axis = [a for a, n in enumerate(rope.sections) for _ in range(n)]
     ang = torch.empty(pos.shape[0], len(step), dtype=torch.float64)
+    whole, half = 1 << TURN, 1 << TURN - 1
     for t, row in enumerate(pos.tolist()):
         for i, st in enumerate(step):
-            frac = (row[rope.axis_of_pair[i]] * st) % 2 ** 64
-            ang[t, i] = (frac if frac < 2 ** 63 else frac - 2 ** 64) * 2.0 ** -64 * 2 * math.pi
+            ang[t, i] = math.ldexp((row[axis[i]] * st + half) % whole - half, -TURN) * 2 * math.pi
     ang = ang.to(x.device)
     c, s = ang.cos()[:, None], ang.sin()[:, None]
     if inverse:

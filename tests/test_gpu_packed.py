@@ -71,6 +71,33 @@ def test_axial_rope_far_positions_strides_and_specials(cuda_dev):
     assert torch.equal(K.axial_rope(x[..., :80], zero, AxialRope((40,))), x[..., :80])
 
 
+@pytest.mark.parametrize("kw", [dict(sections=(32, 32)), dict(sections=(24, 40), layout="half", spectrum="head", theta=5e5),
+                                dict(sections=(4, 8), scale=(0.37, -3.0))])
+def test_rotation_at_any_64_bit_position(cuda_dev, kw):
+    """The angle is that of theta^-e itself, whatever the position: alone, turned back, and behind the norm."""
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    r = AxialRope(**kw)
+    at = [0, 1, -1, 2 ** 31, -2 ** 40 - 7, 2 ** 50 + 1, -2 ** 50, 2 ** 62 + 12345, 2 ** 63 - 1, -2 ** 63, -2 ** 63 + 99]
+    pos = torch.tensor([[a, b] for a in at for b in (at[3], at[-1])], dtype=torch.int64, device=cuda_dev)
+    x = _randn(cuda_dev, 4, len(pos), 3, 128, dtype=F32)
+    for inverse in (False, True):
+        y, size = po.rotate(x.double(), pos, r, inverse=inverse)
+        assert po.within(K.axial_rope(x, pos, r, inverse=inverse), y, po.head_bound(y, size, F32, 128, False)) <= 1
+    y, size = po.rotate(po.norm(x, None, 1e-6), pos, r)
+    for got in K.qk_headnorm_rope(x, x, None, None, 1e-6, pos, r):
+        assert po.within(got, y, po.head_bound(y, size, F32, 128, True)) <= 1
+    near = torch.randint(-2 ** 31, 2 ** 31, (40, 2), generator=_gen(cuda_dev, 1), device=cuda_dev)
+    x = _randn(cuda_dev, 5, 40, 2, 128, dtype=F32)
+    y, size = po.rotate(x.double(), near, r)
+    back, _ = po.rotate(x.double(), near, r, inverse=True)
+    for wide in (1, 0):                                                      # 64 bits of the step do for 32-bit positions
+        r.c.wide = wide
+        for p in (near, near.to(torch.int32)):
+            assert po.within(K.axial_rope(x, p, r), y, po.head_bound(y, size, F32, 128, False)) <= 1
+            assert po.within(K.axial_rope(x, p, r, inverse=True), back, po.head_bound(back, size, F32, 128, False)) <= 1
+
+
 # ---- per-head norm + rotation -------------------------------------------------------------------------------------
 
 

@@ -10,6 +10,7 @@ import torch
 import lbw_b200._lib as L
 import lbw_b200.kernels as K
 import lbw_b200.rope as rope
+import packed_oracle as po
 
 BF = torch.bfloat16
 
@@ -178,3 +179,17 @@ def test_axial_rope_can_be_copied_and_pickled():
     r = rope.AxialRope((8, 4, 4), theta=500.0, layout="half", spectrum="head", scale=(1.0, 0.5, 2.0))
     for c in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
         assert bytes(c.c) == bytes(r.c) and c.scale == r.scale and c.axis_of_pair == r.axis_of_pair
+
+
+@pytest.mark.parametrize("kw", [dict(sections=(22, 21, 21)), dict(sections=(64,), theta=1e6), dict(sections=(3, 5), spectrum="head"),
+                                dict(sections=(8, 4, 4), theta=500.0, scale=(1.0, 0.3, -2.0)),
+                                dict(sections=(8,), theta=0.01, scale=1e9)])
+def test_axial_rope_steps_hold_128_bits_of_the_frequency(kw):
+    """Against theta^-e in 150 digits: the error of an angle is that of the step times the position."""
+    r = rope.AxialRope(**kw)
+    want = po.turns_per_position(r.sections, r.theta, r.spectrum, r.scale)
+    for i, t in enumerate(want):
+        got = r.c.step[i] << 64 | r.c.step_low[i]
+        off = ((got << 64) - t + (1 << 191)) % (1 << 192) - (1 << 191)
+        assert abs(off) <= 1 << 63                                          # half a step of 2^-128 turns
+    assert r.c.wide == 1
