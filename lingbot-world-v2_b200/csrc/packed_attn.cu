@@ -320,9 +320,10 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     // ---------------- scheduler ----------------
     // Takes the next window when the producer loads the last key tile of the present one: about two tiles before its end,
     // enough to hide the answer and the search, and late enough that no CTA holds work which another could start.
-    // Windows come in the grid's order, so the search for a window's sequence goes on where the last one ended.
+    // The search for a window's sequence goes on where the last one ended, as windows mostly come in the grid's order. That
+    // no later answer names an earlier block is promised nowhere: then the search starts again at the first sequence.
     bool have = true;
-    unsigned block = blockIdx.x;
+    unsigned block = blockIdx.x, asked = 0;  // (asked: lane 0's)
     int b_at = 0, loaded = -1;
     unsigned before = 0;  // windows of the sequences before b_at (all counts are below the grid's 2^31)
     PackedSeq s{0, 0, 0, 0};
@@ -330,27 +331,37 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
     for (int i = 0;; ++i) {
       const int slot = i & 1;
       bool ok = true;
-      if (i > 0) {
-        if (lane == 0) {
-          ok = mbar_wait_c(&want_next, (i - 1) & 1, ab, 0x13);
-          if (ok) {
-            mbar_expect_tx(&steal_bar, 16);
-            steal_request(&steal_res, &steal_bar);
-            ok = mbar_wait_c(&steal_bar, (i - 1) & 1, ab, 0x11);
-          }
-          have = ok && steal_answer(&steal_res, block);
-          fence_async_shared();  // (read before the next answer overwrites it)
-        }
-        have = __shfl_sync(0xffffffffu, have, 0);
-        block = __shfl_sync(0xffffffffu, block, 0);
-      }
       PackedWin w;
       w.valid = 0;
-      if (have) {
+      if (i > 0 && lane == 0) ok = mbar_wait_c(&want_next, (i - 1) & 1, ab, 0x13);
+      // The grid is an upper bound: a block past the last window is passed over (a later answer may name one with a window),
+      // and none of them has to start. (3,000 single tokens beside a prompt of 700, whose bound is 6,000 blocks too high:
+      // 262 us, 255 where the other warps left at the first such block.)
+      for (bool ask = i > 0; have && !w.valid; ask = true) {
+        if (ask) {
+          if (lane == 0) {
+            do {
+              if (ok) {
+                mbar_expect_tx(&steal_bar, 16);
+                steal_request(&steal_res, &steal_bar);
+                ok = mbar_wait_c(&steal_bar, asked++ & 1, ab, 0x11);
+              }
+              have = ok && steal_answer(&steal_res, block);
+              fence_async_shared();  // (read before the next answer overwrites it)
+            } while (have && b_at >= a.n_seqs && block / (ta.n_split * ta.head_tiles) >= before);  // (all counted: no window)
+          }
+          have = __shfl_sync(0xffffffffu, have, 0);
+          block = __shfl_sync(0xffffffffu, block, 0);
+          if (!have) break;
+        }
         const unsigned rest = ta.n_split > 1 ? block / ta.n_split : block;
         w.split = (int)(block - rest * ta.n_split);
         const unsigned pair = rest / ta.head_tiles;
         w.head0 = (int)(rest - pair * ta.head_tiles) * ta.pack;
+        if (pair < before) {
+          b_at = 0;
+          before = 0;
+        }
         while (b_at < a.n_seqs) {
           if (loaded != b_at) {  // 32 sequences, one per lane, kept while windows come from them
             const int b = b_at + lane;
@@ -419,17 +430,7 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
         mbar_arrive(&win_full[slot]);
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!w.valid || !ok) {
-        // Past the last window (the grid is an upper bound): take the blocks that are left, so that none has to start.
-        for (int t = i; lane == 0 && have && ok; ++t) {
-          mbar_expect_tx(&steal_bar, 16);
-          steal_request(&steal_res, &steal_bar);
-          if (!mbar_wait_c(&steal_bar, t & 1, ab, 0x12)) break;
-          have = steal_answer(&steal_res, block);
-          fence_async_shared();
-        }
-        break;
-      }
+      if (!w.valid || !ok) break;
     }
   } else if (warp == 16) {
     // ---------------- producer ----------------
