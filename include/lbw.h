@@ -262,7 +262,7 @@ typedef struct {
   int heads, gamma_f32;
 } lbw_head_rows;
 /* out = x rotated, fp32 arithmetic, one rounding; dims beyond 2 * pairs are copied (x->gamma is not used). lbw_dtype
- * `dtype`, head_dim a multiple of 8, at most 256; out may be x, with the same strides. positions: [tokens, axes] int32 or
+ * `dtype`, head_dim a multiple of 8, at most 256; out may be x, with the same strides; else they share no memory. positions: [tokens, axes] int32 or
  * int64 (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does nothing. */
 int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int dtype, const void* positions, int pos_bits,
                    long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream);
@@ -271,7 +271,7 @@ int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int d
  * given, is copied to row k_rows[t] of v->out (a cache of out_rows rows); a row outside [0, out_rows) is not written.
  * Without k_rows the rows are the tokens. Two tokens with the same row leave a mix of both there. The sums of squares are
  * fp32: values beyond 1e18 make them infinite and the head zero. out may be x (k: without k_rows), with the same
- * strides. */
+ * strides; else an output shares no memory with q, k, v (a cache: with all of its rows) or another output. */
 int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const lbw_head_rows* v, long long tokens,
                          int head_dim, int dtype, float eps, const void* positions, int pos_bits, long long pos_tok,
                          long long pos_axis, const lbw_rope_axes* rope, const void* k_rows, int k_rows_bits,
@@ -305,7 +305,7 @@ typedef struct {
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
  * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
  * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels
- * that such a call enqueues). out may be q, with the same strides. */
+ * that such a call enqueues). out may be q, with the same strides; else it shares no memory with q, k or v. */
 int lbw_packed_attention_workspace(long long tq, long long tk, int hq, int hk, int head_dim, int n_seqs, int max_q,
                                    int same_lens, long long* bytes, int* launches);
 int lbw_packed_attention(const lbw_packed_batch* batch, void* workspace, long long ws_bytes, void* stream);

@@ -25,6 +25,7 @@
 
 #include "host_common.cuh"
 #include "lbw_common.cuh"
+#include "overlap.cuh"
 
 namespace lbw {
 
@@ -314,10 +315,29 @@ static int check_seg(const char* who, const char* name, const lbw_head_rows& r, 
   return LBW_OK;
 }
 
-// In place every vector has to stay where it is: others read it. moved: rows go elsewhere.
-static int check_in_place(const char* who, const HeadSeg& g, long long tokens, bool moved) {
-  if (g.x == g.out && (moved || (tokens > 1 && g.xs_tok != g.os_tok) || (g.heads > 1 && g.xs_head != g.os_head)))
-    return set_error(LBW_ERR_INVALID, "%s: in place with other strides or rows", who);
+// Work items read and write in any order, so no output may share memory with an operand, but for its own in place, where every
+// vector has to stay where it is. moved: rows of k and v go elsewhere, to a cache of out_rows.
+static int check_in_place(const char* who, const HeadSeg (&seg)[3], const char* const (&names)[3], long long tokens, int dim,
+                          int dtype, bool moved, long long out_rows) {
+  const int size = dtype == LBW_FP32 ? 4 : 2;
+  ByteGrid in[3], out[3];
+  for (int i = 0; i < 3; ++i) {
+    const HeadSeg& g = seg[i];
+    if (!g.x) continue;
+    const bool away = moved && i > 0;
+    in[i] = ByteGrid::of(g.x, tokens, g.xs_tok, g.heads, g.xs_head, dim, size);
+    out[i] = ByteGrid::of(g.out, away ? out_rows : tokens, g.os_tok, g.heads, g.os_head, dim, size);
+    if (g.x == g.out && (away || (tokens > 1 && g.xs_tok != g.os_tok) || (g.heads > 1 && g.xs_head != g.os_head)))
+      return set_error(LBW_ERR_INVALID, "%s: %s in place with other strides or rows", who, names[i]);
+  }
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 3; ++j) {
+      if (!seg[i].x || !seg[j].x) continue;
+      if (overlap(out[i], in[j]) && !(i == j && seg[i].x == seg[i].out))
+        return set_error(LBW_ERR_INVALID, "%s: the output of %s overlaps %s and is not it in place", who, names[i], names[j]);
+      if (i < j && overlap(out[i], out[j]))
+        return set_error(LBW_ERR_INVALID, "%s: the outputs of %s and %s overlap", who, names[i], names[j]);
+    }
   return LBW_OK;
 }
 
@@ -422,7 +442,7 @@ int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int d
   HeadArgsWide a;
   static_cast<HeadArgs&>(a) = HeadArgs{};
   a.seg[0] = HeadSeg{x->x, x->out, nullptr, x->x_tok, x->x_head, x->out_row, x->out_head, x->heads, 0};
-  if ((err = check_in_place(who, a.seg[0], tokens, false))) return err;
+  if ((err = check_in_place(who, a.seg, {"x", "", ""}, tokens, head_dim, dtype, false, 0))) return err;
   a.tokens = tokens;
   a.dim = head_dim;
   a.pos = positions;
@@ -450,7 +470,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
   HeadArgsWide a;
   static_cast<HeadArgs&>(a) = HeadArgs{};
   const lbw_head_rows* in[3] = {q, k, v};
-  const char* names[3] = {"q", "k", "v"};
+  const char* const names[3] = {"q", "k", "v"};
   for (int i = 0; i < 3; ++i) {
     if (!in[i]) continue;
     const lbw_head_rows& r = *in[i];
@@ -459,8 +479,7 @@ int lbw_qk_headnorm_rope(const lbw_head_rows* q, const lbw_head_rows* k, const l
       return set_error(LBW_ERR_ALIGN, "%s: gamma of %s is misaligned", who, names[i]);
     a.seg[i] = HeadSeg{r.x, r.out, r.gamma, r.x_tok, r.x_head, r.out_row, r.out_head, r.heads, r.gamma_f32};
   }
-  for (int i = 0; i < 3; ++i)
-    if (in[i] && (err = check_in_place(who, a.seg[i], tokens, i > 0 && k_rows))) return err;
+  if ((err = check_in_place(who, a.seg, names, tokens, head_dim, dtype, k_rows != nullptr, out_rows))) return err;
   a.tokens = tokens;
   a.dim = head_dim;
   a.eps = eps;

@@ -37,6 +37,7 @@
 #include <limits.h>
 
 #include "host_common.cuh"
+#include "overlap.cuh"
 #include "packed_common.cuh"
 #include "packed_host.cuh"
 
@@ -1009,9 +1010,14 @@ int lbw_packed_attention(const lbw_packed_batch* batch, void* workspace, long lo
   if (need > 0 && (!workspace || !aligned(workspace, 16) || ws_bytes < need))
     return set_error(LBW_ERR_INVALID, "%s: %lld bytes of 16-byte aligned workspace needed (%lld given)", who, need,
                      ws_bytes);
-  if (tk > 0 && (out == k || out == v)) return set_error(LBW_ERR_INVALID, "%s: out is k or v", who);
-  if (out == q && ((tq > 1 && q_tok != out_tok) || (hq > 1 && q_head != out_head)))
-    return set_error(LBW_ERR_INVALID, "%s: out is q with other strides", who);
+  // Rows are written while others are still computed from q, k and v; a row of out in the place of its own q is not.
+  const ByteGrid o = ByteGrid::of(out, tq, out_tok, hq, out_head, head_dim, 2);
+  if (overlap(o, ByteGrid::of(k, tk, k_tok, hk, k_head, head_dim, 2)) ||
+      overlap(o, ByteGrid::of(v, tk, v_tok, hk, v_head, head_dim, 2)))
+    return set_error(LBW_ERR_INVALID, "%s: out is k or v, or overlaps them", who);
+  if (out == q ? (tq > 1 && q_tok != out_tok) || (hq > 1 && q_head != out_head)
+               : overlap(o, ByteGrid::of(q, tq, q_tok, hq, q_head, head_dim, 2)))
+    return set_error(LBW_ERR_INVALID, "%s: out is q with other strides, or overlaps it", who);
   int* st = device_status(&err);
   if (!st) return err;
   const PackedArgs a{cu_q, cu_k, k_lens, n_seqs, (int)tq, (int)tk, hq, hk, hq / hk, causal != 0,

@@ -193,3 +193,25 @@ def test_axial_rope_steps_hold_128_bits_of_the_frequency(kw):
         off = ((got << 64) - t + (1 << 191)) % (1 << 192) - (1 << 191)
         assert abs(off) <= 1 << 63                                          # half a step of 2^-128 turns
     assert r.c.wide == 1
+
+
+def test_outputs_that_overlap_an_operand_are_refused(lib):
+    """Not only at the same address: later rows, other heads, rows of the cache, and the other operands' outputs."""
+    axial = dict(x=P, x_tok=128, x_head=64, out=ctypes.c_void_p(4096 + 256), out_tok=128, out_head=64, tokens=5, heads=2, dim=64,
+                 dtype=0, pos=P, bits=32, pos_tok=1, pos_axis=1, rope=_rope(), inverse=0)
+    for change in ({}, dict(out=ctypes.c_void_p(4096 - 256)), dict(x_tok=256, out_tok=256, out=ctypes.c_void_p(4096 + 128))):
+        assert _axial(lib, {**axial, **change}) == L.LBW_ERR_INVALID and "overlaps x" in L.last_error()
+    near = lambda at, out, **kw: _rows(x=at, out=out, x_tok=128, out_row=128, **kw)   # noqa: E731 (5 rows: 1,280 bytes)
+    a, b, c, d = (1 << 20 + i for i in range(4))
+    for q, k, v, rows, say in (
+            (near(a, b), near(b, c), None, None, "q overlaps k"), (near(a, a), near(a, c), None, None, "q overlaps k"),
+            (near(a, c), near(b, c + 256), None, None, "outputs of q and k"), (near(a, c), near(b, a + 1024), None, None, "k overlaps q"),
+            (near(a, a), near(b + 256 * 8, b), None, P, "k overlaps k"),          # a cache row in use as the new keys
+            (near(a, a), near(b, c), near(c + 256 * 39, d), P, "k overlaps v"), (near(a, a), near(b, c), near(d, c + 512), P, "outputs of k")):
+        assert lib.lbw_qk_headnorm_rope(q, k, v, 5, 64, 0, 1e-6, P, 32, 1, 1, _rope(), rows, 64, 40, None) == L.LBW_ERR_INVALID
+        assert say in L.last_error(), L.last_error()
+    far = ctypes.c_void_p(1 << 30)
+    at = ctypes.c_void_p((1 << 20) + 2 * 1024 * 99)                                # the last of the 100 rows
+    for name in "qkv":
+        one = {**dict(q=far, k=far, v=far), name: ctypes.c_void_p(1 << 20), "out": at}
+        assert _packed(lib, {**CALL, **one}) == L.LBW_ERR_INVALID and "overlaps" in L.last_error()
