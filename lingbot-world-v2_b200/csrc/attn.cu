@@ -343,13 +343,14 @@ __global__ void __launch_bounds__(attn::THREADS, 1)
     }
   } else if (warp == 10) {
     // ---------------- K/V watcher ----------------
-    // Observes every landing in order (K(0) first), so none of its parity waits runs a phase ahead, and waits for
-    // each p_ready[0][h] phase to complete before arriving for the next key tile: an early arrival would count
-    // toward the current phase and release P V before every softmax thread had written its part of P.
+    // Waits for each p_ready[0][h] phase to complete before arriving for the next key tile: an early arrival would
+    // count toward the current phase and release P V before every softmax thread had written its part of P. That also
+    // keeps its parity waits in step: the landings before the one it waits for were needed for the P it has seen, and
+    // the ring slot is not loaded again before its own arrival. K(0) has no arrival behind it: S(0) and the load of
+    // K(2) into its slot go on without the watcher, which could be lapped if it waited for K(0), and needs not.
     if (lane == 0) {
       const int n_tiles = g_end - g_begin;
-      bool ok = mbar_wait(&k_full[0], 0, ab, 0x60);
-      for (int j = 0; j < n_tiles && ok; ++j) {
+      for (int j = 0; j < n_tiles; ++j) {
         if (!mbar_wait(&v_full[j & 1], (j >> 1) & 1, ab, 0x61)) break;
         mbar_arrive(&p_ready[0][0]);
         if (j + 1 < n_tiles && !mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, ab, 0x62)) break;

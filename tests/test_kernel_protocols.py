@@ -8,8 +8,7 @@ Attention:
 
 The programs restate the kernel's synchronisation, step for step:
   producer   Q once; per key tile j: wait k_empty[j % 2] (use j / 2), load K; wait v_empty, load V
-  watcher    K(0) landed; per tile j: V(j) landed -> arrive p_ready[0][0]; K(j + 1) landed -> arrive p_ready[0][1];
-             then wait for both phases of tile j to complete (so its next arrivals cannot land in them)
+  watcher    per tile j: V(j) landed -> arrive p_ready[0][0]; K(j + 1) landed -> arrive p_ready[0][1]; then wait for both phases of tile j to complete (so its next arrivals cannot land in them)
   issuer     S_0 = Q_0 K_0^T (and S_1 with two query tiles), commit s_full; commit k_empty[0]; per tile j:
              wait p_ready[0][0] (P_0 keys 0..63 and V(j)) -> P_0 V (keys 0..63); wait p_ready[0][1] (P_0 keys
              64..127 and K(j + 1)) -> P_0 V (keys 64..127); next S_0, commit s_full[0]; then the same P_1 V for the
@@ -48,7 +47,7 @@ import pytest
 from protocol_model import Bar, Flag, Model
 
 
-def attention_v1(m, n_tiles, two, rescale_p, ragged_p, watcher_phase_wait=True):
+def attention_v1(m, n_tiles, two, rescale_p, ragged_p, watcher_phase_wait=True, watch_first_k=False, lateness=0.0):
     nq = 2 if two else 1
     q_full = Bar("q_full")
     k_full, k_empty = [Bar(f"k_full{s}") for s in range(2)], [Bar(f"k_empty{s}") for s in range(2)]
@@ -77,7 +76,10 @@ def attention_v1(m, n_tiles, two, rescale_p, ragged_p, watcher_phase_wait=True):
             yield ("tma", v_full[s], ("V", j))
 
     def watcher():
-        yield ("wait", k_full[0], 1)             # every landing observed in order, K(0) first
+        if lateness:                             # instructions that are not in the cache yet
+            yield ("work", m.rng.uniform(0, lateness))
+        if watch_first_k:
+            yield ("wait", k_full[0], 1)
         for j in range(n_tiles):
             yield ("wait", v_full[j & 1], (j >> 1) + 1)
             assert p_ready[0][0].k == j, ("watcher arrival in another phase", j)
@@ -171,6 +173,23 @@ def test_attention_protocol_random_schedules(jitter):
         attention_v1(m, n_tiles=rng.randint(1, 7), two=rng.random() < 0.7, rescale_p=rng.choice([0.0, 0.3, 1.0]),
                      ragged_p=rng.choice([0.0, 0.5]))
         m.run()
+
+
+@pytest.mark.parametrize("watch_first_k", [False, True])
+def test_attention_watcher_may_start_late(watch_first_k):
+    """Nothing that the watcher waits for can be lapped, however late it starts. K(0) could: S(0) and the load of K(2) into
+    the same slot do not depend on it, and a watcher that waited for K(0) after that would wait for good."""
+    caught = 0
+    for seed in range(200):
+        rng = random.Random(seed)
+        m = Model(seed)
+        attention_v1(m, n_tiles=rng.randint(1, 7), two=rng.random() < 0.7, rescale_p=0.3, ragged_p=0.5,
+                     watch_first_k=watch_first_k, lateness=8000.0)
+        try:
+            m.run()
+        except AssertionError:
+            caught += 1
+    assert caught > 0 if watch_first_k else caught == 0
 
 
 def test_model_catches_a_watcher_running_ahead():
