@@ -15,11 +15,12 @@ TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}   # 
 def attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, scale=None):
     """(out, bound) [tq, hq, d] fp64; rows of no sequence are NaN in both.
 
-    out = sum_j p_j v_j / sum_j p_j. A probability is off by u where it is rounded for the second product, by 1.9e-4
-    where its exponential is (the cubic on the FMA pipe, 1.8e-4; ex2.approx is below 2^-21), and by the error s of its
-    score, |q|.|k| scale times 2^-23 for each of the d products summed in fp32 (2^-23: sums may be cut, not rounded); the
-    sum of probabilities has the same without u, and the second product's n additions cost 2^-23 each. A rounded
-    probability below the fp16 normals is off by 2^-25 at most, with the largest at least 2^-8."""
+    out = sum_j p_j v_j / sum_j p_j. A probability is off by u where it is rounded for the second product, by 2^-21 where its
+    exponential is (ex2.approx), and by the error s of its score, |q|.|k| scale times 2^-23 for each of the d products summed
+    in fp32 (2^-23: sums may be cut, not rounded); the sum of probabilities has the same without u, and the second product's
+    n additions cost 2^-23 each. A probability below the fp16 normals is off by 2^-25 at most where it is rounded, against a
+    sum of 1 or more: the maximum that is subtracted is never above the row's largest score, whose probability is then 1 or
+    more (with the keys in ranges this holds for the range of the largest maximum, and the others are scaled down to it)."""
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     group = q.shape[1] // k.shape[1]
     out = torch.full(q.shape, float("nan"), dtype=torch.float64, device=q.device)
@@ -50,8 +51,8 @@ def attention(q, k, v, cu_q, cu_k, k_lens=None, causal=True, scale=None):
         o = (p @ vv) / total
         spread = (p @ vv.abs()) / total                                                  # sum p |v| / sum p
         s = mag.amax(-1, keepdim=True) * qq.shape[-1] * 2.0 ** -23
-        rel = u + 2 * 1.9e-4 + 2.2 * s + n * 2.0 ** -23
-        low = n * tiny * 2.0 ** 8 * vv.abs().amax() if tiny else 0.0
+        rel = u + 2 * 2.0 ** -21 + 2.2 * s + n * 2.0 ** -23
+        low = n * tiny * vv.abs().amax() if tiny else 0.0
         empty = torch.isinf(top) & (top < 0)
         out[cq[b]:cq[b + 1]] = torch.where(empty, torch.zeros((), dtype=torch.float64, device=q.device), o).transpose(0, 1)
         bound[cq[b]:cq[b + 1]] = torch.where(empty, torch.zeros((), dtype=torch.float64, device=q.device),
