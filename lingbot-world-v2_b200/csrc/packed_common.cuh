@@ -70,13 +70,13 @@ LBW_DEV int packed_visible(const PackedArgs& a, const PackedSeq& s, int i) {
 }
 
 // The whole block of NT threads: an item of a list in which sequence b has n.x items (SEARCH_Y: n.y) of (n.x, n.y) =
-// count(b); which(sums over all sequences) says which item. Returns its sequence, its index in it, both sums before the
-// sequence and over all; seq = -1 past the end. Each thread counts a run of neighbouring sequences, and one thread's
+// count(b); which(sum of all n.y) says which item. Returns its sequence, its index in it, the sum of n.y before the
+// sequence and that over all; seq = -1 past the end. Each thread counts a run of neighbouring sequences, and one thread's
 // reading of the found sequence is what all get. `tmp`: NT / 32 entries of shared memory.
 struct PackedAt {
   int seq;
   PackedSeq sq;
-  long long local, before_x, before_y, total_x, total_y;
+  long long local, before_y, total_y;
 };
 
 template <int NT, bool SEARCH_Y, typename F, typename W>
@@ -84,16 +84,16 @@ LBW_DEV PackedAt packed_locate(const PackedArgs& a, F count, W which, longlong2*
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = (a.n_seqs + NT - 1) / NT;
   const int b0 = (int)min((long long)threadIdx.x * per, (long long)a.n_seqs), b1 = min(b0 + per, a.n_seqs);
-  long long x = 0, y = 0;
+  long long x = 0, y = 0;  // (x only for a search by n.x)
   for (int b = b0; b < b1; ++b) {
     const longlong2 n = count(b);
-    x += n.x;
+    if constexpr (!SEARCH_Y) x += n.x;
     y += n.y;
   }
   long long sx = x, sy = y;  // inclusive over the warp
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long vx = __shfl_up_sync(0xffffffffu, sx, o), vy = __shfl_up_sync(0xffffffffu, sy, o);
+    const long long vx = SEARCH_Y ? 0 : __shfl_up_sync(0xffffffffu, sx, o), vy = __shfl_up_sync(0xffffffffu, sy, o);
     if (lane >= o) {
       sx += vx;
       sy += vy;
@@ -102,7 +102,7 @@ LBW_DEV PackedAt packed_locate(const PackedArgs& a, F count, W which, longlong2*
   if (lane == 31) tmp[warp] = make_longlong2(sx, sy);
   if (threadIdx.x == 0) at->seq = -1;
   __syncthreads();
-  long long tx = 0, ty = 0;
+  long long ty = 0;
   sx -= x;
   sy -= y;
 #pragma unroll
@@ -112,10 +112,9 @@ LBW_DEV PackedAt packed_locate(const PackedArgs& a, F count, W which, longlong2*
       sx += v.x;
       sy += v.y;
     }
-    tx += v.x;
     ty += v.y;
   }
-  const long long w = which(make_longlong2(tx, ty));
+  const long long w = which(ty);
   long long from = SEARCH_Y ? sy : sx;
   if (w >= from && w < from + (SEARCH_Y ? y : x)) {
     for (int b = b0; b < b1; ++b) {
@@ -125,18 +124,15 @@ LBW_DEV PackedAt packed_locate(const PackedArgs& a, F count, W which, longlong2*
         at->seq = b;
         at->sq = packed_seq(a, b);
         at->local = w - from;
-        at->before_x = sx;
         at->before_y = sy;
         break;
       }
       from += own;
-      sx += n.x;
       sy += n.y;
     }
   }
   __syncthreads();
   PackedAt r = *at;
-  r.total_x = tx;
   r.total_y = ty;
   return r;
 }

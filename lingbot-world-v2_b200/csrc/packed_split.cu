@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(ps::THREADS, 1)
   }
   const PackedAt at = packed_locate<THREADS, true>(
       a, [&](int b) { return split_count(a, max_rows, b); },
-      [&](longlong2 total) { return (long long)blockIdx.x * split_share(total.y, gridDim.x); }, tmp, &at_s);
+      [&](long long total) { return (long long)blockIdx.x * split_share(total, gridDim.x); }, tmp, &at_s);
   const long long share = split_share(at.total_y, gridDim.x);
   const long long first = blockIdx.x * share;
   pdl_trigger();
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(128) packed_join_kernel(const __grid_constant_
   __shared__ PackedAt at_s;
   __shared__ float s_acc[4][D], s_l[4];
   const PackedAt at = packed_locate<128, false>(
-      a, [&](int b) { return split_count(a, max_rows, b); }, [&](longlong2) { return (long long)blockIdx.x; }, tmp,
+      a, [&](int b) { return split_count(a, max_rows, b); }, [&](long long) { return (long long)blockIdx.x; }, tmp,
       &at_s);
   pdl_wait();
   if (at.seq < 0) return;
