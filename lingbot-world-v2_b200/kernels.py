@@ -790,7 +790,8 @@ def _rows3(who, name, form, dtype=None, dim=None, written=False):
         raise ValueError(f"{who}: {name} needs a contiguous head_dim")
     if written and ((stride[0] == 0 and shape[0] > 1) or (stride[1] == 0 and shape[1] > 1)):
         raise ValueError(f"{who}: {name} is an expanded tensor")
-    return (*shape, stride[0], stride[1])
+    # (torch leaves any stride on a dimension of size 1; it is never used, and need not be aligned)
+    return (*shape, stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0)
 
 
 def _positions(who, form, tokens, axes):

@@ -611,3 +611,27 @@ def test_compiled_graph_equals_eager(cuda_dev):
         return K.packed_attention(K.axial_rope(q, pos, rope), k, qkv[:, 4:], cu, cu)
 
     assert torch.equal(torch.compile(f, fullgraph=True, backend="aot_eager")(qkv, pos, cu), f(qkv, pos, cu))
+
+
+def test_strides_of_a_dimension_of_one(cuda_dev):
+    """Whatever stride torch leaves on a dimension of size 1 (here: 1), it is never used and nothing is refused for it."""
+    import lbw_b200.kernels as K
+    from lbw_b200.rope import AxialRope
+    rope = AxialRope((32,))
+    flat = _randn(cuda_dev, 1, 9, 64)
+    for x in (flat[:, :, None].transpose(1, 2), flat[:1, :, None].permute(2, 0, 1), flat.t().contiguous().t()[:, None][:1].contiguous()):
+        x = x if x.shape[1:] == (1, 64) else x.transpose(0, 1)
+        n = x.shape[0]
+        plain = x.contiguous().view(-1).clone().view(n, 1, 64)
+        pos, cu = torch.arange(n, device=cuda_dev), _cu([n], cuda_dev)
+        want = K.axial_rope(plain, pos, rope)
+        assert torch.equal(K.axial_rope(x, pos, rope), want)
+        out = torch.empty(n, 64, 1, dtype=BF, device=cuda_dev).transpose(1, 2)
+        assert out.stride(1) == 1 and torch.equal(K.axial_rope(x, pos, rope, out=out), want)
+        for a, b in zip(K.qk_headnorm_rope(x, x, None, None, 1e-6, pos, rope), K.qk_headnorm_rope(plain, plain, None, None, 1e-6, pos, rope)):
+            assert torch.equal(a, b)
+        want = K.packed_attention(plain, plain, plain, cu, cu)
+        assert torch.equal(K.packed_attention(x, x, x, cu, cu, out=out), want)
+        for q in (x[:1], x[-1:].as_strided((1, 1, 64), (3, 1, 1), x[-1:].storage_offset())):
+            one = _cu([1], cuda_dev)
+            assert torch.equal(K.packed_attention(q, x, x, one, cu), K.packed_attention(q.contiguous().clone(), plain, plain, one, cu))

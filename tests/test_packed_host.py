@@ -215,3 +215,10 @@ def test_outputs_that_overlap_an_operand_are_refused(lib):
     for name in "qkv":
         one = {**dict(q=far, k=far, v=far), name: ctypes.c_void_p(1 << 20), "out": at}
         assert _packed(lib, {**CALL, **one}) == L.LBW_ERR_INVALID and "overlaps" in L.last_error()
+
+
+def test_strides_of_a_dimension_of_one_are_not_passed_on():
+    x = torch.zeros(5, 64, 1).transpose(1, 2)
+    assert x.stride() == (64, 1, 1) and K._rows3("op", "x", K._form(x)) == (5, 1, 64, 64, 0)
+    x = torch.zeros(2, 64).as_strided((1, 2, 64), (3, 64, 1))
+    assert K._rows3("op", "x", K._form(x)) == (1, 2, 64, 0, 64)
