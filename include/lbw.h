@@ -300,8 +300,9 @@ typedef struct {
  * the tensors are cut to what does.
  * q, out: [tq, hq, head_dim]; k, v: [tk, hk, head_dim]; hq (at most 65,536) a multiple of hk, query head h uses kv head
  * h / (hq / hk); tq * hq and tk below 2^31 - 1,024; head_dim 64 or 128; dtype LBW_BF16 or LBW_FP16 for all four. A value
- * that is not finite makes its column infinite or NaN in the rows that see it, a NaN key all of such a row; no other row
- * is touched.
+ * that is not finite makes its column infinite or NaN in the rows that see it; a key that gives a row the score NaN or
+ * +infinity makes all of that row NaN, one with the score -infinity takes no part in it (nothing but such scores: zeros, as
+ * where no key is seen). No other row is touched.
  * max_q: the largest number of queries of a sequence if the caller knows it (0: not known); it chooses kernels only.
  * workspace: lbw_packed_attention_workspace bytes, 16-byte aligned, not shared by calls that may overlap (same_lens
  * != 0: for calls that pass one array as cu_q and cu_k, and no k_lens; launches, if not NULL, gets the number of kernels

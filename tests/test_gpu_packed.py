@@ -635,3 +635,24 @@ def test_strides_of_a_dimension_of_one(cuda_dev):
         for q in (x[:1], x[-1:].as_strided((1, 1, 64), (3, 1, 1), x[-1:].storage_offset())):
             one = _cu([1], cuda_dev)
             assert torch.equal(K.packed_attention(q, x, x, one, cu), K.packed_attention(q.contiguous().clone(), plain, plain, one, cu))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,n", [(1, 700), (4, 300), (4, 40), (300, 300), (40, 6000)])
+def test_packed_attention_infinite_scores(cuda_dev, q_len, n, dim, dtype):
+    """A score of -inf takes no part, a row of nothing else is zeros, a score of +inf makes its row NaN."""
+    import lbw_b200.kernels as K
+    q, k, v, cu_q, cu_k = _attention_case(cuda_dev, 5, [q_len], [n], 4, 2, dim, dtype)
+    q[..., 3] = q[..., 3].abs() + 0.1
+    gone = torch.zeros(n, dtype=torch.bool, device=cuda_dev)
+    gone[1::3], gone[n // 2:n // 2 + 150] = True, True                      # (a whole key tile among them)
+    k[gone, :, 3] = -math.inf
+    want, bound = po.attention(q, k[~gone], v[~gone], cu_q, _cu([int((~gone).sum())], cuda_dev), causal=False)
+    out = K.packed_attention(q, k, v, cu_q, cu_k, causal=False)
+    assert po.within(out, want, bound) <= 1
+    k[n // 3 // 3 * 3, 1, 3] = math.inf                                     # seen by the heads of the second kv head
+    out = K.packed_attention(q, k, v, cu_q, cu_k, causal=False)
+    assert torch.isnan(out[:, 2:].float()).all() and po.within(out[:, :2], want[:, :2], bound[:, :2]) <= 1
+    k[..., 3] = -math.inf
+    assert bool((K.packed_attention(q, k, v, cu_q, cu_k, causal=False) == 0).all())
