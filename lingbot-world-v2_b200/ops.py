@@ -244,7 +244,8 @@ def _(a, a_s, w, w_s, bias, fmt):
 
 OPS = ("chunk_attention", "chunk_attention_partial", "chunk_attention_tail", "attention_merge", "layernorm_mod", "layernorm_mod_mx",
        "layernorm_affine_mx", "qkv_proj", "rmsnorm_rope", "qk_rmsnorm_rope", "linear_residual", "linear_rowss", "linear_gelu",
-       "mx_linear_gelu", "mx_linear_residual", "mx_quantize_into", "mx_quantize", "mx_linear")
+       "mx_linear_gelu", "mx_linear_residual", "mx_quantize_into", "mx_quantize", "mx_linear", "axial_rope",
+       "qk_headnorm_rope", "packed_attention")
 
 
 @functools.lru_cache(None)

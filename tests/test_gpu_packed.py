@@ -656,3 +656,70 @@ def test_packed_attention_infinite_scores(cuda_dev, q_len, n, dim, dtype):
     assert torch.isnan(out[:, 2:].float()).all() and po.within(out[:, :2], want[:, :2], bound[:, :2]) <= 1
     k[..., 3] = -math.inf
     assert bool((K.packed_attention(q, k, v, cu_q, cu_k, causal=False) == 0).all())
+
+
+AXES = ([16, 16], 10000.0, "half", "axis", [1.0, 1.0])
+
+
+def _opcheck_args(name, dev):
+    qkv = _randn(dev, 1, 50, 6, 64)
+    q, k, v = (qkv[:, :2].contiguous(), qkv[:, 2:4].contiguous(), qkv[:, 4:].contiguous())
+    pos, cu = torch.arange(100, device=dev).view(50, 2), _cu([20, 30], dev)
+    if name == "axial_rope":
+        return q, pos, *AXES, False, torch.empty_like(q)
+    if name == "packed_attention":
+        return q, k, v, cu, cu.clone(), torch.tensor([15, 30], dtype=torch.int32, device=dev), True, 0.125, torch.empty_like(q), 30
+    caches = [torch.zeros(70, 2, 64, dtype=BF, device=dev) for _ in range(2)]
+    return (q, k, _randn(dev, 2, 64), _randn(dev, 3, 64, dtype=F32), 1e-6, pos, *AXES, torch.empty_like(q), caches[0], v, caches[1],
+            torch.arange(50, device=dev) + 10)
+
+
+@pytest.mark.parametrize("name", ["axial_rope", "qk_headnorm_rope", "packed_attention"])
+def test_packed_operators_opcheck(cuda_dev, name):
+    """The tensors that an operator declares it writes are the ones it writes; compiled with dynamic shapes it does the same."""
+    import lbw_b200.ops as O
+    assert name in O.OPS
+    res = torch.library.opcheck(getattr(torch.ops.lbw, name), _opcheck_args(name, cuda_dev),
+                                test_utils=("test_schema", "test_faketensor", "test_aot_dispatch_dynamic"), raise_exception=False)
+    assert all(v == "SUCCESS" for v in res.values()), res
+
+
+def test_compiled_step_over_a_cache_equals_eager(cuda_dev):
+    """A layer's middle in one graph: norm and rotation in place inside the fused tensor or to cache rows, lengths of the
+    sequences in use, the output in the query's place; caches, rows and lengths that change between the calls."""
+    import lbw_b200.kernels as K
+    import lbw_b200.ops  # noqa: F401
+    from lbw_b200.rope import AxialRope
+    hq, hk, d, cap = 8, 2, 64, 90
+    rope = AxialRope((16, 16))
+    gain = _randn(cuda_dev, 9, d)
+
+    def step(qkv, pos, rows, kc, vc, cu_q, cu_k, k_lens):
+        q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+        qo, _ = K.qk_headnorm_rope(q, k, gain, None, 1e-6, pos, rope, q_out=q, k_out=kc, v=v, v_out=vc, k_rows=rows)
+        return K.packed_attention(qo, kc, vc, cu_q, cu_k, k_lens=k_lens, out=qo, max_q=40)
+
+    def prompt(qkv, pos, cu):
+        q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+        K.qk_headnorm_rope(q, k, gain, gain, 1e-6, pos, rope, q_out=q, k_out=k)
+        return K.axial_rope(K.packed_attention(q, k, v, cu, cu, causal=False), pos, rope, inverse=True)
+
+    torch._dynamo.reset()
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    both = [[torch.zeros(2 * cap, hk, d, dtype=BF, device=cuda_dev) for _ in range(2)] for _ in range(2)]
+    done = [0, 0]
+    for i, new in enumerate(([40, 7], [1, 1], [1, 1], [3, 1])):
+        at = torch.cat([torch.arange(done[b], done[b] + n) + b * cap for b, n in enumerate(new)]).to(cuda_dev)
+        done = [a + n for a, n in zip(done, new)]
+        pos = torch.stack([at, at * 3], 1)
+        cu_q, cu_k = _cu(new, cuda_dev), _cu([cap, cap], cuda_dev)
+        k_lens = torch.tensor(done, dtype=torch.int32, device=cuda_dev)
+        qkv = [_randn(cuda_dev, i, sum(new), hq + 2 * hk, d) for _ in range(2)]
+        with torch.no_grad():
+            out = [f(x, pos, at, *c, cu_q, cu_k, k_lens) for f, x, c in zip((step, compiled), qkv, both)]
+        assert torch.equal(*out) and torch.equal(*qkv)
+        assert torch.equal(both[0][0], both[1][0]) and torch.equal(both[0][1], both[1][1])
+    qkv = [_randn(cuda_dev, 8, 47, hq + 2 * hk, d) for _ in range(2)]
+    pos, cu = torch.arange(94, device=cuda_dev).view(47, 2), _cu([40, 7], cuda_dev)
+    assert torch.equal(prompt(qkv[0], pos, cu), torch.compile(prompt, fullgraph=True, backend="aot_eager")(qkv[1], pos, cu))
+    assert torch.equal(*qkv)
