@@ -2,7 +2,8 @@
 // with grouped heads, the sequences' starts and lengths read from device memory (lbw_packed_attention).
 //
 // Online softmax over 128-key tiles, fp32 scores, maxima, sums and accumulators; the probabilities are rounded once to
-// the tensors' 16-bit type for the second product (half a step of 2^-8 or 2^-11 each, averaged over the keys).
+// the tensors' 16-bit type for the second product (off by 2^-8 or 2^-11 of themselves at most, in fp16 by 2^-25 where they are
+// below 2^-14; the row's largest is 1 or more), while their sum takes them unrounded.
 //
 // A CTA has up to two tiles of 128 query rows of one kv head. A row is a (token, query head) pair: `pack` query heads of
 // the kv head's group sit side by side in a tile (row = token * pack + head), so that a tile of a short sequence is
@@ -64,8 +65,9 @@ struct TileArgs {
 
 // tcgen05 operations of a converged warp, issued by one of its lanes. Which: for D = 128 the elected one (always the same),
 // elected in each operation's own asm; for D = 64 lane 0, by the predicate `lead`. A predicated MMA takes the issuer 79
-// cycles, an elected one 65, and one runs for 64 (32 where D = 64 is its N). Measured (us, elected / predicated): D = 128
-// 10,800 causal tokens 1,032 / 1,070, 64 x 300..900 359 / 372; D = 64 16,000 tokens 1,545 / 1,405, 8 x 1,000 63 / 59.
+// cycles, an elected one 65, and one runs for 64 (32 where D = 64 is its N). Measured (us, this rule / the other way round;
+// bf16, replayed from a graph, the same inputs): D = 128 causal, 10,800 tokens of 40 / 8 heads 969 / 969, 64 x 300..900 of
+// 16 / 2 heads 163 / 175; D = 64 without a mask, 16,000 tokens of 8 heads 834 / 857, 8 x 1,000 of 16 heads 68.1 / 68.6.
 template <bool ELECT>
 LBW_DEV void mma_f16_ss_one(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
   if constexpr (ELECT)
@@ -369,6 +371,8 @@ __global__ void __launch_bounds__(pa::THREADS, 1)
             s = b < a.n_seqs ? packed_seq(a, b) : PackedSeq{0, 0, 0, 0};
             if (a.n_seqs > 1) {
               // Those with most keys first: their windows are the longest, and a CTA that took one last would be alone.
+              // Measured (us, so / in the batch's order, as above): 256 x 64..300 tokens of 16 / 2 heads 141.1 / 144.5, three
+              // clips of 1,560 to 4,680 111.5 / 112.8, 48 x 1..509 of 32 / 8 90.0 / 90.8, 64 x 300..900 163.3 / 162.7.
               int rank = 0;
 #pragma unroll
               for (int o = 0; o < 32; ++o) {
