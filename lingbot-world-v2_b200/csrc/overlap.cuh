@@ -23,6 +23,7 @@ struct ByteGrid {
 
   // Strides not negative, s0 the larger, dimensions that repeat or continue the inner ones folded into len.
   void tidy() {
+    if (n0 < 1 || n1 < 1) return;  // no bytes at all
     if (s0 < 0) base += s0 * (n0 - 1), s0 = -s0;
     if (s1 < 0) base += s1 * (n1 - 1), s1 = -s1;
     if (s0 == 0) n0 = 1;

@@ -723,3 +723,10 @@ def test_compiled_step_over_a_cache_equals_eager(cuda_dev):
     pos, cu = torch.arange(94, device=cuda_dev).view(47, 2), _cu([40, 7], cuda_dev)
     assert torch.equal(prompt(qkv[0], pos, cu), torch.compile(prompt, fullgraph=True, backend="aot_eager")(qkv[1], pos, cu))
     assert torch.equal(*qkv)
+
+
+def test_an_empty_operand_overlaps_nothing(cuda_dev):
+    """Keys and values of no rows at the output's own address: nothing to read there."""
+    import lbw_b200.kernels as K
+    x, cu = _randn(cuda_dev, 1, 4, 2, 64), _cu([4], cuda_dev)
+    assert bool((K.packed_attention(x, x[:0], x[:0], cu, cu * 0, out=x) == 0).all())

@@ -64,4 +64,6 @@ def test_slices_of_one_buffer(meet):
     assert meet(cache, ((1 << 20) + 2 * 8 * 8 * d, 4, 8 * d, 8, d, d, 2))       # rows 8 .. 11
     assert not meet(cache, ((1 << 20) + 2 * 5000 * 8 * d, 4, 8 * d, 8, d, d, 2))
     assert not meet((0, 0, w, 8, d, d, 2), cache)                              # no rows
+    for empty in ((1 << 20, 0, 0, 8, d, d, 2), (1 << 20, 0, 0, 1, 0, d, 2), (1 << 20, 0, -w, 8, 0, d, 2), (1 << 20, 5, w, 0, 0, d, 2)):
+        assert not meet(empty, cache) and not meet(cache, empty)               # whatever its strides
     assert not meet((4096, t, w, 40, d, d, 2), (4096 + 2 * 40 * d, t // 2, 2 * w, 8, d, d, 2))   # other strides, between
