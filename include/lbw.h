@@ -262,8 +262,9 @@ typedef struct {
   int heads, gamma_f32;
 } lbw_head_rows;
 /* out = x rotated, fp32 arithmetic, one rounding; dims beyond 2 * pairs are copied (x->gamma is not used). lbw_dtype
- * `dtype`, head_dim a multiple of 8, at most 256; out may be x, with the same strides; else they share no memory. positions: [tokens, axes] int32 or
- * int64 (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does nothing. */
+ * `dtype`, head_dim a multiple of 8, at most 256; out may be x, with the same strides, else they share no memory.
+ * positions: [tokens, axes] int32 or int64 (pos_bits), any values. inverse != 0 turns the other way. tokens = 0 does
+ * nothing. */
 int lbw_axial_rope(const lbw_head_rows* x, long long tokens, int head_dim, int dtype, const void* positions, int pos_bits,
                    long long pos_tok, long long pos_axis, const lbw_rope_axes* rope, int inverse, void* stream);
 /* Every head vector of q and k: x * rsqrt(mean(x^2) + eps) * gamma, then the rotation (rope NULL: none), fp32 with one
